@@ -22,7 +22,11 @@ ext = CUDAExtension(
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
-        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950"],
+        # packed fp32 instructions are off: some of their forms have given
+        # wrong results now and then
+        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
+                 "-Xclang", "-target-feature", "-Xclang",
+                 "-packed-fp32-ops"],
     },
 )
 
