@@ -1,0 +1,131 @@
+// Torch bindings of the 8-bit products (int8.hip). Everything that a kernel
+// takes for granted about its operands is checked here, before the launch.
+
+#include <hip/hip_runtime.h>
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+
+extern "C" {
+void launch_quantize_rows(const void*, int, long, long, long, int8_t*, long,
+                          float*, hipStream_t);
+long int8_product_workspace(long, long, long);
+void launch_int8_product(const int8_t*, long, const float*, const int8_t*,
+                         long, const float*, const float*, long, long, long,
+                         void*, int, int*, hipStream_t);
+}
+
+namespace {
+
+int type_id(torch::ScalarType t) {
+  switch (t) {
+    case torch::kFloat32: return 0;
+    case torch::kFloat16: return 1;
+    case torch::kBFloat16: return 2;
+    default:
+      TORCH_CHECK(false, "unsupported type ", t,
+                  ": float32, float16 or bfloat16 is wanted");
+  }
+}
+
+hipStream_t stream_of(const torch::Tensor& t) {
+  return at::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+// x [m, k], rows contiguous -> (q [m, k] with rows at multiples of 16 bytes,
+// scale [m])
+std::tuple<torch::Tensor, torch::Tensor> quantize_rows(torch::Tensor x) {
+  TORCH_CHECK(x.is_cuda(), "x must be on the GPU");
+  TORCH_CHECK(x.dim() == 2, "x must be 2-D");
+  const int type = type_id(x.scalar_type());
+  const c10::DeviceGuard guard(x.device());
+  const long m = x.size(0), k = x.size(1);
+  TORCH_CHECK(m < (1L << 31) && k < (1L << 31), "x is too large");
+  if (k > 1 && x.stride(1) != 1) x = x.contiguous();
+  const long padded = (k + 15) / 16 * 16;
+  auto q = torch::empty({m, padded}, x.options().dtype(torch::kInt8));
+  auto scale = torch::empty({m}, x.options().dtype(torch::kFloat32));
+  if (m > 0 && k > 0)
+    launch_quantize_rows(x.data_ptr(), type, m, k, x.stride(0),
+                         q.data_ptr<int8_t>(), padded,
+                         scale.data_ptr<float>(), stream_of(x));
+  else
+    scale.zero_();
+  return {q.narrow(1, 0, k), scale};
+}
+
+// Rows that begin at multiples of 16 bytes; others are copied. A kernel reads
+// 16 bytes at a time, up to 15 of them behind a row's last value; as they are
+// aligned they lie in the same page.
+torch::Tensor aligned_rows(const torch::Tensor& q) {
+  const long k = q.size(1);
+  const bool fine = (k <= 1 || q.stride(1) == 1) &&
+                    (q.size(0) == 1 ||
+                     (q.stride(0) % 16 == 0 && q.stride(0) >= k &&
+                      q.stride(0) < (1L << 23))) &&
+                    (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) == 0;
+  if (fine) return q;
+  auto rows = torch::empty({q.size(0), (k + 15) / 16 * 16}, q.options());
+  auto view = rows.narrow(1, 0, k);
+  view.copy_(q);
+  return view;
+}
+
+torch::Tensor int8_product(torch::Tensor xq, torch::Tensor xs,
+                           torch::Tensor wq, torch::Tensor ws,
+                           c10::optional<torch::Tensor> bias,
+                           torch::ScalarType out_type) {
+  TORCH_CHECK(xq.is_cuda(), "xq must be on the GPU");
+  TORCH_CHECK(xq.dim() == 2 && wq.dim() == 2 && xq.size(1) == wq.size(1),
+              "xq and wq must be [m, k] and [n, k]");
+  TORCH_CHECK(xq.dtype() == torch::kInt8 && wq.dtype() == torch::kInt8,
+              "xq and wq must be int8");
+  const long m = xq.size(0), n = wq.size(0), k = xq.size(1);
+  // 131071 products of at most 128^2 fit in 32 bits
+  TORCH_CHECK(k < 131072, "k must be below 131072, so that the sums fit in "
+              "32 bits (got ", k, ")");
+  TORCH_CHECK(m < (1L << 31) - 256 && n < (1L << 31) - 256,
+              "xq or wq has too many rows");
+  auto scale = [&](const torch::Tensor& t, long size, const char* name) {
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == size &&
+                t.dtype() == torch::kFloat32 && t.device() == xq.device(),
+                name, " must be float32 of ", size, " values on xq's device");
+    return t.contiguous();
+  };
+  TORCH_CHECK(wq.device() == xq.device(), "wq must be on xq's device");
+  const c10::DeviceGuard guard(xq.device());
+  xs = scale(xs, m, "x_scale");
+  ws = scale(ws, n, "w_scale");
+  torch::Tensor b;
+  if (bias.has_value()) b = scale(*bias, n, "bias");
+  const int type = type_id(out_type);
+  auto out = torch::empty({m, n}, xq.options().dtype(out_type));
+  if (m == 0 || n == 0) return out;
+  if (k == 0) {
+    if (b.defined()) out.copy_(b.expand({m, n})); else out.zero_();
+    return out;
+  }
+  xq = aligned_rows(xq);
+  wq = aligned_rows(wq);
+  torch::Tensor work;
+  if (const long size = int8_product_workspace(m, n, k))
+    work = torch::empty({size}, xq.options().dtype(torch::kInt32));
+  const long one = (k + 15) / 16 * 16;  // a single row's stride says nothing
+  launch_int8_product(xq.data_ptr<int8_t>(), m == 1 ? one : xq.stride(0),
+                      xs.data_ptr<float>(), wq.data_ptr<int8_t>(),
+                      n == 1 ? one : wq.stride(0), ws.data_ptr<float>(),
+                      b.defined() ? b.data_ptr<float>() : nullptr, m, n, k,
+                      out.data_ptr(), type,
+                      work.defined() ? work.data_ptr<int>() : nullptr,
+                      stream_of(xq));
+  return out;
+}
+
+}  // namespace
+
+void register_int8(py::module_& mod) {
+  mod.def("quantize_rows", &quantize_rows,
+          "8-bit rows and the scale of each");
+  mod.def("int8_product", &int8_product,
+          "product of 8-bit matrices with a scale for each row and column");
+}

@@ -19,6 +19,7 @@ from .reductions import col_moments, col_minmax, col_sum, merge_moments
 from .glm import glm_value_grad
 from .kmeans import kmeans_assign, closest_center
 from .elementwise import affine_transform
+from .int8 import int8_linear, int8_matmul, quantize_rows
 
 __all__ = [
     "col_moments",
@@ -29,4 +30,7 @@ __all__ = [
     "kmeans_assign",
     "closest_center",
     "affine_transform",
+    "int8_linear",
+    "int8_matmul",
+    "quantize_rows",
 ]

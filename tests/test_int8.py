@@ -1,0 +1,367 @@
+"""8-bit rows and their products: the CPU form against 64-bit arithmetic and
+the refusals here, the HIP kernels against the CPU form with -m gpu."""
+
+import math
+
+import pytest
+import torch
+
+from mi355ml import ops
+from mi355ml.ops.int8 import MAX_K
+
+FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _rows(m, k, dtype=torch.float32, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g) * torch.exp(
+        torch.randn(m, 1, generator=g))
+    return x.to(dtype)
+
+
+def _int8(m, k, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-128, 128, (m, k), generator=g).to(torch.int8)
+
+
+def _expect_quantized(x):
+    """The definition with Python's own exact arithmetic."""
+    from fractions import Fraction
+    qs, ss = [], []
+    for row in x.double().tolist():
+        big = max((abs(v) for v in row), default=0.0)
+        s = torch.tensor(big / 127, dtype=torch.float64).float().item()
+        ss.append(s)
+        qs.append([max(-127, min(127, round(Fraction(v) / Fraction(s))))
+                   if s > 0 else 0 for v in row])
+    return qs, ss
+
+
+def _halves(dtype):
+    """Rows whose values lie on and next to the middle of two integers."""
+    x = torch.tensor([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, 3.5, 126.5],
+                      [254.0, 1.0, 3.0, 5.0, -1.0, -3.0, -253.0, 7.0]])
+    if dtype == torch.float32:
+        near = torch.nextafter(x, torch.full_like(x, 1e9))
+        near[:, 0] = x[:, 0]
+        below = torch.nextafter(x, torch.full_like(x, -1e9))
+        below[:, 0] = x[:, 0]
+        g = torch.Generator().manual_seed(3)
+        # a scale that is no power of two, and values around its halves
+        s = torch.tensor(0.0123456789)
+        n = torch.arange(-126, 126).float() + 0.5
+        odd = torch.cat([(s * 127)[None], (s * n),
+                         torch.nextafter(s * n, torch.tensor(9.0)),
+                         torch.nextafter(s * n, torch.tensor(-9.0))])
+        wide = odd[torch.randperm(len(odd), generator=g)]
+        pad = torch.zeros(6, len(wide))
+        pad[0], pad[1, :8], pad[2, :8] = wide, x[0], x[1]
+        pad[3, :8], pad[4, :8], pad[5, :8] = near[0], below[0], near[1]
+        return pad
+    return x.to(dtype)
+
+
+def _same(x, device="cpu"):
+    q, s = ops.quantize_rows(x.to(device))
+    want_q, want_s = _expect_quantized(x)
+    assert q.dtype == torch.int8 and s.dtype == torch.float32
+    assert q.shape == x.shape and s.shape == x.shape[:1]
+    assert q.stride(0) % 16 == 0 or device == "cpu"
+    assert q.cpu().tolist() == want_q
+    assert s.cpu().tolist() == want_s
+
+
+def _edges(device):
+    x = torch.zeros(7, 21)
+    x[0, 3] = float("nan")
+    x[1, 20] = float("-inf")
+    x[1, 0] = 1.0
+    x[3] = torch.linspace(-1e-45, 3e-43, 21)        # subnormal, so is s
+    x[4] = torch.linspace(-1, 1, 21) * 3e38
+    x[5, 7] = -1e-46                                # rounds to zero
+    x[6] = torch.linspace(-1e-35, 2e-36, 21)
+    q, s = ops.quantize_rows(x.to(device))
+    q, s = q.cpu(), s.cpu()
+    assert math.isnan(s[0]) and math.isnan(s[1])
+    assert not q[:2].any()
+    assert s[2] == 0 and not q[2].any() and s[5] == 0
+    want_q, want_s = _expect_quantized(x[3:])
+    assert q[3:].tolist() == want_q and s[3:].tolist() == want_s
+    assert q.abs().max() == 127
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_quantize_definition(dtype):
+    _same(_rows(9, 37, dtype))
+    _same(_halves(dtype))
+
+
+def test_quantize_edges():
+    _edges("cpu")
+
+
+def test_quantize_error_is_half_a_scale():
+    x = _rows(50, 200)
+    q, s = ops.quantize_rows(x)
+    off = (q.double() * s.double()[:, None] - x.double()).abs()
+    assert (off <= s.double()[:, None] / 2).all()
+
+
+@pytest.mark.parametrize("shape", [(0, 5), (5, 0), (0, 0), (1, 1)])
+def test_quantize_small(shape):
+    q, s = ops.quantize_rows(torch.ones(shape))
+    assert q.shape == shape and s.shape == shape[:1]
+
+
+def _product_expected(xq, xs, wq, ws, bias):
+    y = xq.double() @ wq.double().t()
+    y = y * xs.double()[:, None] * ws.double()[None, :]
+    size = y.abs()
+    if bias is not None:
+        y = y + bias.double()
+        size = size + bias.double().abs()
+    return y, size
+
+
+def _check_product(m, n, k, dtype, bias=True, device="cpu", shift=0):
+    xq, wq = _int8(m, k + shift, 1)[:, shift:], _int8(n, k, 2)
+    g = torch.Generator().manual_seed(5)
+    xs, ws = torch.rand(m, generator=g), torch.rand(n, generator=g)
+    b = torch.randn(n, generator=g) * 100 if bias else None
+    want, size = _product_expected(xq, xs, wq, ws, b)
+    args = [None if t is None else t.to(device) for t in (xq, xs, wq, ws, b)]
+    got = ops.int8_matmul(*args, out_dtype=dtype)
+    assert got.dtype == dtype and got.shape == (m, n)
+    # the sum to float32, two scales, the bias: four roundings in float32 of
+    # values no larger than `size`, and one to the output's type
+    half = torch.finfo(torch.float32).eps / 2
+    far = 4 * half * size * (1 + 8 * half)
+    far = far + torch.finfo(dtype).eps / 2 * (want.abs() + far)
+    # below the normal range half a step is the same for all values
+    far = far + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    got = got.cpu().double()
+    fits = want.abs() < torch.finfo(dtype).max * 0.999
+    assert ((got - want).abs() <= far)[fits].all()
+    assert (got.abs() >= torch.finfo(dtype).max * 0.998)[~fits].all()
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (3, 5, 17), (20, 7, 1000)])
+def test_product(m, n, k, dtype):
+    _check_product(m, n, k, dtype)
+    _check_product(m, n, k, dtype, bias=False)
+
+
+def test_product_largest_sums_are_exact():
+    q = torch.full((2, MAX_K), -128, dtype=torch.int8)
+    one = torch.ones(2)
+    y = ops.int8_matmul(q, one, q, one)
+    assert (y == float(MAX_K * 16384)).all()
+
+
+def test_linear_is_quantize_then_product():
+    x, w = _rows(13, 50, torch.bfloat16), _rows(6, 50)
+    wq, ws = ops.quantize_rows(w)
+    b = torch.randn(6)
+    got = ops.int8_linear(x, wq, ws, b)
+    xq, xs = ops.quantize_rows(x)
+    assert got.dtype == torch.bfloat16
+    assert torch.equal(got, ops.int8_matmul(xq, xs, wq, ws, b,
+                                            torch.bfloat16))
+
+
+def test_bad_rows_give_nan_alone():
+    x, w = _rows(5, 30), _rows(4, 30)
+    x[1, 2], x[3, 0] = float("inf"), float("nan")
+    wq, ws = ops.quantize_rows(w)
+    y = ops.int8_linear(x, wq, ws)
+    assert y[[1, 3]].isnan().all() and y[[0, 2, 4]].isfinite().all()
+
+
+def test_refusals():
+    x = torch.ones(4, 8)
+    q, s = ops.quantize_rows(x)
+    with pytest.raises(ValueError, match="2-D"):
+        ops.quantize_rows(torch.ones(3))
+    with pytest.raises(TypeError, match="float32"):
+        ops.quantize_rows(torch.ones(3, 3, dtype=torch.float64))
+    with pytest.raises(TypeError, match="int8"):
+        ops.int8_matmul(x, s, q, s)
+    with pytest.raises(ValueError, match="rows of"):
+        ops.int8_matmul(q, s, q[:, :4], s)
+    with pytest.raises(ValueError, match="x_scale"):
+        ops.int8_matmul(q, s[:2], q, s)
+    with pytest.raises(ValueError, match="bias"):
+        ops.int8_matmul(q, s, q, s, torch.ones(5))
+    with pytest.raises(TypeError, match="w_scale"):
+        ops.int8_matmul(q, s, q, s.double())
+    with pytest.raises(TypeError, match="out_dtype"):
+        ops.int8_matmul(q, s, q, s, out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="w_scale"):
+        ops.int8_matmul(q, s, q, s.to("meta"))
+    long = torch.zeros(1, MAX_K + 1, dtype=torch.int8)
+    with pytest.raises(ValueError, match="overflow"):
+        ops.int8_matmul(long, s[:1], long, s[:1])
+    with pytest.raises(TypeError, match="float32"):
+        ops.int8_linear(torch.ones(3, 3, dtype=torch.int32), q, s)
+
+
+# ------------------------------------------------------------------ GPU
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_gpu_quantize_definition(dtype):
+    _same(_halves(dtype), "cuda")
+    for m, k in [(1, 1), (3, 15), (5, 16), (2, 17), (130, 100), (7, 129)]:
+        _same(_rows(m, k, dtype, seed=k), "cuda")
+
+
+@pytest.mark.gpu
+def test_gpu_quantize_edges():
+    _edges("cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("k", [250, 257, 511, 600, 1025, 2047, 4100, 8192,
+                               8209, 16385, 50001])
+def test_gpu_quantize_row_lengths(k, dtype):
+    x = _rows(5, k, dtype, seed=k)
+    q, s = ops.quantize_rows(x)
+    gq, gs = ops.quantize_rows(x.cuda())
+    assert torch.equal(gq.cpu(), q) and torch.equal(gs.cpu(), s)
+    # the filling behind the row is zeros
+    rows = gq.as_strided((5, gq.stride(0)), (gq.stride(0), 1))
+    assert not rows[:, k:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_gpu_quantize_strides(dtype):
+    x = _rows(40, 300, dtype)
+    for view in (lambda t: t[:, 1:], lambda t: t[3:, 7:290],
+                 lambda t: t[::2, :255], lambda t: t.t(),
+                 lambda t: t[:, ::3], lambda t: t[:1].expand(6, -1)):
+        q, s = ops.quantize_rows(view(x))
+        gq, gs = ops.quantize_rows(view(x.cuda()))
+        assert torch.equal(gq.cpu(), q) and torch.equal(gs.cpu(), s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0, 5), (5, 0), (0, 0)])
+def test_gpu_empty(shape):
+    q, s = ops.quantize_rows(torch.ones(shape, device="cuda"))
+    assert q.shape == shape and s.shape == shape[:1] and not s.any()
+    w = torch.zeros(3, shape[1], dtype=torch.int8, device="cuda")
+    ws, b = torch.ones(3, device="cuda"), torch.arange(3.0, device="cuda")
+    y = ops.int8_matmul(q, s, w, ws, b)
+    assert y.shape == (shape[0], 3) and torch.equal(
+        y, b.expand(shape[0], 3))
+    assert ops.int8_matmul(q, s, w[:0], ws[:0]).shape == (shape[0], 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2, 15, 16, 17, 33, 64, 65, 127, 200, 300])
+@pytest.mark.parametrize("n,k", [(1, 1), (5, 16), (50, 100), (16, 127),
+                                 (33, 129), (130, 640), (257, 2065)])
+def test_gpu_product(m, n, k):
+    _check_product(m, n, k, torch.float32, device="cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("m,n,k", [(3, 40, 300), (70, 41, 300),
+                                   (2100, 2050, 200), (4, 17, 50000),
+                                   (500, 60, 20001)])
+def test_gpu_product_types(m, n, k, dtype):
+    _check_product(m, n, k, dtype, device="cuda")
+    _check_product(m, n, k, dtype, bias=False, device="cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 90])
+def test_gpu_product_rows_that_are_not_aligned(m):
+    for k in (31, 100, 256):
+        for shift in (0, 1, 4):
+            _check_product(m, 20, k, torch.float32, device="cuda",
+                           shift=shift)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 90])
+def test_gpu_product_does_not_read_behind_its_columns(m):
+    # columns of a wider matrix: what stands behind them must not count
+    q = _int8(m, 256, 7)
+    w = _int8(20, 256, 8)
+    one, two = torch.ones(m), torch.ones(20)
+    for k in (1, 50, 128, 130, 255):
+        want, _ = _product_expected(q[:, :k], one, w[:, :k], two, None)
+        got = ops.int8_matmul(q.cuda()[:, :k], one.cuda(), w.cuda()[:, :k],
+                              two.cuda())
+        assert torch.equal(got.cpu().double(), want)
+
+
+@pytest.mark.gpu
+def test_gpu_product_largest_sums_are_exact():
+    for m in (2, 80):
+        q = torch.full((m, MAX_K), -128, dtype=torch.int8, device="cuda")
+        one = torch.ones(m, device="cuda")
+        y = ops.int8_matmul(q, one, q, one)
+        assert (y == float(MAX_K * 16384)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 20, 100])
+def test_gpu_linear(m):
+    for dtype in FLOATS:
+        x, w = _rows(m, 500, dtype), _rows(77, 500)
+        wq, ws = ops.quantize_rows(w)
+        b = torch.randn(77)
+        want = ops.int8_linear(x, wq, ws, b, torch.float32)
+        got = ops.int8_linear(x.cuda(), wq.cuda(), ws.cuda(), b.cuda(),
+                              torch.float32)
+        xq, xs = ops.quantize_rows(x)
+        _, size = _product_expected(xq, xs, wq, ws, b)
+        # both sides have the same integers; each makes at most four
+        # roundings in float32
+        half = torch.finfo(torch.float32).eps / 2
+        assert ((got.cpu() - want).double().abs() <= 9 * half * size).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [2, 100])
+def test_gpu_bad_rows_give_nan_alone(m):
+    x, w = _rows(m, 30), _rows(4, 30)
+    x[1, 2] = float("nan")
+    wq, ws = ops.quantize_rows(w.cuda())
+    y = ops.int8_linear(x.cuda(), wq, ws)
+    assert y[1].isnan().all() and y.isnan().sum() == 4
+
+
+@pytest.mark.gpu
+def test_gpu_other_stream_and_graph():
+    x, w = _rows(300, 2000).cuda(), _rows(70, 2000).cuda()
+    wq, ws = ops.quantize_rows(w)
+    want = [ops.int8_linear(x[:m], wq, ws) for m in (5, 300)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [ops.int8_linear(x[:m], wq, ws) for m in (5, 300)]
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    static = x.clone()
+    graphs = []
+    for m in (5, 300):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.int8_linear(static[:m], wq, ws)
+        graphs.append((graph, out, m))
+    for seed in range(4):
+        new = _rows(300, 2000, seed=seed + 10).cuda()
+        static.copy_(new)
+        for graph, _, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out, m in graphs:
+            assert torch.equal(out, ops.int8_linear(new[:m], wq, ws))
