@@ -248,9 +248,11 @@ torch::Tensor affine_transform(torch::Tensor x, torch::Tensor a,
 }  // namespace
 
 void register_int8(py::module_& mod);  // bindings_int8.cpp
+void register_orthogonalize(py::module_& mod);  // bindings_orthogonalize.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   register_int8(mod);
+  register_orthogonalize(mod);
   mod.def("col_moments_partial", &col_moments_partial,
           "per-WG column (n, sum, M2) partials");
   mod.def("col_minmax_partial", &col_minmax_partial,

@@ -1,0 +1,310 @@
+// Torch bindings of the Newton-Schulz orthogonalisation (orthogonalize.hip).
+// Everything that a kernel takes for granted about its operands is checked
+// here, before the launch.
+
+#include <hip/hip_runtime.h>
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+
+#include <cmath>
+
+#include "orthogonalize.h"
+
+extern "C" {
+int gram_parts(long, int, int);
+void launch_gram(const void*, int, int, long, int, long, long, int, double*,
+                 int, double*, hipStream_t);
+void launch_factor(const double*, int, int, double, double, double, int,
+                   double*, hipStream_t);
+void launch_apply(const void*, int, int, long, int, long, long, int,
+                  const double*, void*, long, long, hipStream_t);
+void launch_split(const void*, int, int, int, long, long, int, double*, int,
+                  Halves, Halves, float*, hipStream_t);
+void launch_step(Halves, int, Halves, int, int, int, Step, int, int,
+                 hipStream_t);
+}
+
+namespace {
+
+constexpr long kGramMost = 128;  // longest shorter side of the Gram way
+
+struct Matrices {
+  torch::Tensor x;
+  int type;      // 0 float32, 1 float16, 2 bfloat16
+  long batch, rows, cols, ld, stride;
+  bool wide;     // fewer rows than columns
+  long length;   // the longer side
+  int n;         // the shorter one
+};
+
+Matrices matrices_of(torch::Tensor x) {
+  TORCH_CHECK(x.is_cuda(), "x must be on the GPU");
+  TORCH_CHECK(x.dim() == 2 || x.dim() == 3, "x must be 2-D or 3-D");
+  Matrices v;
+  switch (x.scalar_type()) {
+    case torch::kFloat32: v.type = 0; break;
+    case torch::kFloat16: v.type = 1; break;
+    case torch::kBFloat16: v.type = 2; break;
+    default: TORCH_CHECK(false, "unsupported type ", x.scalar_type());
+  }
+  v.batch = x.dim() == 3 ? x.size(0) : 1;
+  v.rows = x.size(-2);
+  v.cols = x.size(-1);
+  TORCH_CHECK(v.batch < 65536, "at most 65535 matrices at a time");
+  if ((v.cols > 1 && x.stride(-1) != 1) ||
+      (v.rows > 1 && x.stride(-2) < v.cols))
+    x = x.contiguous();
+  v.x = x;
+  v.ld = v.rows > 1 ? x.stride(-2) : v.cols;
+  v.stride = x.dim() == 3 ? x.stride(0) : 0;
+  v.wide = v.rows < v.cols;
+  v.length = std::max(v.rows, v.cols);
+  v.n = (int)std::min(v.rows, v.cols);
+  return v;
+}
+
+hipStream_t stream_of(const torch::Tensor& t) {
+  return at::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+torch::TensorOptions doubles(const torch::Tensor& t) {
+  return t.options().dtype(torch::kFloat64);
+}
+
+// The upper 16 x 16 tiles of X X^T of the shorter side, [batch, tiles * 256].
+torch::Tensor gram_of(const Matrices& v) {
+  const long nt = (v.n + 15) / 16, size = nt * (nt + 1) / 2 * 256;
+  const int parts = gram_parts(v.length, v.n, (int)v.batch);
+  auto gram = torch::empty({v.batch, size}, doubles(v.x));
+  torch::Tensor slab;
+  if (parts > 1) slab = torch::empty({v.batch, parts, size}, doubles(v.x));
+  launch_gram(v.x.data_ptr(), v.type, v.wide, v.length, v.n, v.ld, v.stride,
+              (int)v.batch, parts > 1 ? slab.data_ptr<double>() : nullptr,
+              parts, gram.data_ptr<double>(), stream_of(v.x));
+  return gram;
+}
+
+torch::Tensor factor_of(const torch::Tensor& gram, long n, long steps,
+                        double a, double b, double c) {
+  const long nt = (n + 15) / 16;
+  auto q = torch::empty({gram.size(0), nt * 16, nt * 16}, gram.options());
+  launch_factor(gram.data_ptr<double>(), (int)n, (int)steps, a, b, c,
+                (int)gram.size(0), q.data_ptr<double>(), stream_of(gram));
+  return q;
+}
+
+torch::Tensor apply_to(const Matrices& v, const torch::Tensor& q) {
+  auto out = torch::empty(v.x.sizes(), v.x.options());
+  launch_apply(v.x.data_ptr(), v.type, v.wide, v.length, v.n, v.ld, v.stride,
+               (int)v.batch, q.data_ptr<double>(), out.data_ptr(), v.cols,
+               v.rows * v.cols, stream_of(v.x));
+  return out;
+}
+
+// Which power of two brings values of magnitude up to `most` below 2^15.
+int shift_for(double most) {
+  if (!(most > 0)) return 0;
+  int e;
+  std::frexp(most, &e);
+  return std::max(-60, std::min(60, 15 - e));
+}
+
+double pow2(int e) { return std::ldexp(1.0, e); }
+
+// The largest |b l + c l^2| for 0 <= l <= top.
+double largest_of_b(double b, double c, double top) {
+  double most = std::abs(b * top + c * top * top);
+  if (c != 0) {
+    const double l = -b / (2 * c);
+    if (l > 0 && l < top) most = std::max(most, std::abs(b * l + c * l * l));
+  }
+  return most;
+}
+
+// The largest |a s + b s^3 + c s^5| for 0 <= s <= top.
+double largest_of_step(double a, double b, double c, double top) {
+  auto at = [&](double s) {
+    const double l = s * s;
+    return std::abs(s * (a + l * (b + c * l)));
+  };
+  double most = at(top);
+  auto consider = [&](double l) {
+    if (l > 0 && l < top * top) most = std::max(most, at(std::sqrt(l)));
+  };
+  // a + 3 b l + 5 c l^2 = 0
+  if (c == 0) {
+    if (b != 0) consider(-a / (3 * b));
+  } else {
+    const double d = 9 * b * b - 20 * a * c;
+    if (d >= 0) {
+      consider((-3 * b + std::sqrt(d)) / (10 * c));
+      consider((-3 * b - std::sqrt(d)) / (10 * c));
+    }
+  }
+  return most;
+}
+
+// How many of the three products hi hi, hi lo, lo hi a matrix product takes.
+// float32 and float16 results take all three everywhere: about 2^-22 for each
+// product. A bfloat16 result is rounded to 2^-9, and there one product is
+// enough for G and G^2, whose rounding in 11 bits acts on large and small
+// singular values alike. The product with X needs X itself in full (an error
+// in a large singular direction that leaks into a small one is raised with it
+// by a in every later step), except in the last step, which nothing follows.
+// On gradient-like matrices (a few strong directions over noise) that leaves
+// an error of 3e-4 to 1.6e-3 of the norm before the result's own rounding
+// (1.7e-3); a single product everywhere left 4e-3 to 2e-2.
+struct Precision {
+  int gram, square, step, first, last;
+};
+
+torch::Tensor by_products(const Matrices& v, int steps, double a, double b,
+                          double c) {
+  const Precision precise = {3, 3, 3, 3, 3}, brief = {1, 1, 2, 1, 1};
+  const Precision& p = v.type == 2 ? brief : precise;
+  const long n = v.n, m = v.length, batch = v.batch;
+  const long np = (n + 63) / 64 * 64, mp = (m + 63) / 64 * 64;
+  TORCH_CHECK(m <= (1L << 23), "the longer side may have at most 2^23 values "
+              "where the shorter one has more than ", kGramMost);
+  const auto halves = v.x.options().dtype(torch::kFloat16);
+  auto matrix = [&](std::vector<torch::Tensor>& keep, long rows, long ld) {
+    keep.push_back(torch::empty({2, batch, rows, ld}, halves));
+    auto* hi = (unsigned short*)keep.back().data_ptr();
+    return Halves{hi, hi + batch * rows * ld, ld, rows * ld};
+  };
+  std::vector<torch::Tensor> keep;
+  const Halves x = matrix(keep, n, mp);
+  Halves xt = matrix(keep, m, np), xt_next = matrix(keep, m, np);
+  const Halves g = matrix(keep, n, np);
+  Halves poly = matrix(keep, n, np);
+  if (p.step < 3) poly.lo = nullptr;
+  const int parts = 256;
+  auto squares = torch::empty({batch, parts}, doubles(v.x));
+  auto factor = torch::empty({batch}, v.x.options().dtype(torch::kFloat32));
+  auto out = torch::empty(v.x.sizes(), v.x.options());
+  const auto st = stream_of(v.x);
+  launch_split(v.x.data_ptr(), v.type, (int)v.rows, (int)v.cols, v.ld,
+               v.stride, (int)batch, squares.data_ptr<double>(), parts, x, xt,
+               factor.data_ptr<float>(), st);
+
+  double bound = 1.0;  // of the singular values of X
+  int ex = 14;         // stored values are 2^ex times the true ones
+  for (int k = 0; k < steps; ++k) {
+    const bool last = k + 1 == steps;
+    const double top = bound * bound * 1.01;
+    const int eg = shift_for(top);
+    const int ep = shift_for(largest_of_b(b, c, top) * 1.01);
+    bound = largest_of_step(a, b, c, bound * 1.005) * 1.01;
+    // float32 holds the values in between up to here with room to spare
+    TORCH_CHECK(bound < 1e12, "the coefficients let the iteration diverge");
+    if (!(bound > 0)) bound = 1e-6;
+    const int next = last ? 0 : shift_for(bound);
+
+    Step s = {};
+    s.factor = factor.data_ptr<float>();
+    s.d = s.t = g;
+    s.alpha = (float)pow2(eg - 2 * ex);
+    s.power = k == 0 ? 2 : 0;
+    s.symmetric = 1;
+    launch_step(x, (int)n, x, (int)n, (int)m, p.gram, s, (int)batch, 0, st);
+
+    s.d = s.t = poly;
+    s.e = g;
+    s.alpha = (float)(c * pow2(ep - 2 * eg));
+    s.beta = (float)(b * pow2(ep - eg));
+    s.power = 0;
+    launch_step(g, (int)n, g, (int)n, (int)n, p.square, s, (int)batch, 0, st);
+
+    s = Step{};
+    s.factor = factor.data_ptr<float>();
+    s.power = k == 0 ? 1 : 0;
+    s.e = x;
+    s.alpha = (float)pow2(next - ep - ex);
+    s.beta = (float)(a * pow2(next - ex));
+    if (last) {
+      s.out = out.data_ptr();
+      s.ld_out = v.cols;
+      s.batch_out = v.rows * v.cols;
+      s.tall = v.rows > v.cols;
+    } else {
+      s.d = x;
+      s.t = xt_next;
+    }
+    launch_step(poly, (int)n, xt, (int)m, (int)n,
+                last ? p.last : k == 0 ? p.first : p.step, s, (int)batch,
+                last ? 1 + v.type : 0, st);
+    std::swap(xt, xt_next);
+    ex = next;
+  }
+  return out;
+}
+
+void check_steps(long steps, double a, double b, double c) {
+  TORCH_CHECK(steps >= 1 && steps <= 1000, "steps must be 1 to 1000");
+  TORCH_CHECK(std::isfinite(a) && std::isfinite(b) && std::isfinite(c),
+              "coefficients must be finite");
+}
+
+torch::Tensor newton_schulz(torch::Tensor x, long steps, double a, double b,
+                            double c) {
+  check_steps(steps, a, b, c);
+  const c10::DeviceGuard guard(x.device());
+  const Matrices v = matrices_of(x);
+  if (x.numel() == 0) return torch::empty(x.sizes(), x.options());
+  if (v.n <= kGramMost)
+    return apply_to(v, factor_of(gram_of(v), v.n, steps, a, b, c));
+  return by_products(v, (int)steps, a, b, c);
+}
+
+// The Gram way in its three parts, for a panel whose rows are spread over
+// ranks: the sum of the ranks' Gram tiles is the whole panel's.
+void check_panel(const torch::Tensor& x) {
+  TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1 && x.size(1) <= kGramMost,
+              "a panel must be 2-D with 1 to ", kGramMost, " columns");
+}
+
+Matrices panel_of(const torch::Tensor& x) {
+  Matrices v = matrices_of(x);
+  v.wide = false;
+  v.length = v.rows;
+  v.n = (int)v.cols;
+  return v;
+}
+
+torch::Tensor panel_gram(torch::Tensor x) {
+  check_panel(x);
+  const c10::DeviceGuard guard(x.device());
+  const Matrices v = panel_of(x);
+  if (v.rows == 0) {
+    const long nt = (v.n + 15) / 16;
+    return torch::zeros({nt * (nt + 1) / 2 * 256}, doubles(x));
+  }
+  return gram_of(v)[0];
+}
+
+torch::Tensor panel_finish(torch::Tensor x, torch::Tensor gram, long steps,
+                           double a, double b, double c) {
+  check_steps(steps, a, b, c);
+  check_panel(x);
+  const c10::DeviceGuard guard(x.device());
+  const Matrices v = panel_of(x);
+  const long nt = (v.n + 15) / 16;
+  TORCH_CHECK(gram.dim() == 1 && gram.is_contiguous() &&
+              gram.dtype() == torch::kFloat64 &&
+              gram.size(0) == nt * (nt + 1) / 2 * 256 &&
+              gram.device() == x.device(), "gram is not what panel_gram gives");
+  if (v.rows == 0) return torch::empty(x.sizes(), x.options());
+  return apply_to(v, factor_of(gram.unsqueeze(0), v.n, steps, a, b, c));
+}
+
+}  // namespace
+
+void register_orthogonalize(py::module_& mod) {
+  mod.def("newton_schulz", &newton_schulz,
+          "orthogonalise matrices by Newton-Schulz products");
+  mod.def("panel_gram", &panel_gram,
+          "64-bit Gram matrix of a panel, its upper tiles");
+  mod.def("panel_finish", &panel_finish,
+          "orthogonalise a panel whose Gram matrix is known");
+}

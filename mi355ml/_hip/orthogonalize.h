@@ -1,0 +1,24 @@
+// What orthogonalize.hip and bindings_orthogonalize.cpp pass to each other.
+#pragma once
+
+// A matrix as hi + lo, two fp16 numbers a value (lo may be null: hi alone),
+// rows of ld values, a multiple of 64, zeros behind the last.
+struct Halves {
+  unsigned short* hi;
+  unsigned short* lo;
+  long ld, batch;  // in values
+};
+
+// What a product is made into: v = (alpha C + beta E) factor^power.
+struct Step {
+  Halves e;          // E; hi null: none
+  Halves d, t;       // v as halves, and its transpose; hi null: not wanted
+  void* out;         // or v in the type of the result
+  long ld_out, batch_out;
+  int tall;          // the result holds the transpose of v
+  float alpha, beta;
+  const float* factor;  // a value for each matrix of the batch
+  int power;
+  int symmetric;     // v is, and its lower tiles are computed alone
+  int tm, tn;        // tiles (set by the launch)
+};

@@ -1,0 +1,743 @@
+// Orthogonalising a matrix by Newton-Schulz products:
+//
+//   X_0 = X / ||X||_F,   X <- a X + (b G + c G^2) X,   G = X X^T
+//
+// with the Gram matrix G of the shorter side n (X is n x m here, n <= m; a
+// tall matrix is taken as its transpose). The singular vectors stay, each
+// singular value goes through s <- a s + b s^3 + c s^5.
+//
+// Two ways, by the length of the shorter side:
+//
+// n <= 128: everything happens on the Gram matrix. X_k = Q_k X_0 where Q_k is
+//   a polynomial in G_0, and G_{k+1} = P G_k P, Q_{k+1} = P Q_k with
+//   P = a + b G_k + c G_k^2. So X is read for G_0, and once more for Q X,
+//   whatever the number of steps. G_0 squares the singular values, and the
+//   steps raise the smallest of them by up to a^steps; 64-bit products
+//   (v_mfma_f64_16x16x4_f64) keep that harmless, at a cost that hides behind
+//   the memory for the panels of 64 columns that a range finder makes.
+//
+// n > 128: the products as they stand, on the 16-bit matrix cores. As X_0 has
+//   norm 1, all values have known bounds, and a fixed power of two brings
+//   them into the range of fp16. A value is held as hi + lo, two fp16 numbers
+//   that give 22 bits together, and a product takes hi hi + hi lo + lo hi:
+//   close to float32's precision at a third of the fp16 rate, which is still
+//   several times the rate of float32. bindings_orthogonalize.cpp says what
+//   16-bit results can do without (Precision).
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "orthogonalize.h"
+#include "tile_product.h"
+
+using namespace tile_product;
+
+namespace {
+
+typedef double v4d __attribute__((ext_vector_type(4)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+
+// v_mfma_f64_16x16x4_f64: a lane gives row (column) lane % 16 of the first
+// (second) operand at k = lane / 16, and has rows 4 i + lane / 16 of column
+// lane % 16 of the result.
+__device__ __forceinline__ v4d mma64(double x, double y, v4d c) {
+  return __builtin_amdgcn_mfma_f64_16x16x4f64(x, y, c, 0, 0, 0);
+}
+
+// Tile (i, j), i <= j, of the upper triangle of nt x nt tiles.
+__host__ __device__ constexpr int upper(int nt, int i, int j) {
+  return i * nt - i * (i - 1) / 2 + (j - i);
+}
+
+template <class T> struct Four {
+  struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[4]; };
+};
+
+// Element (p, q) of a panel stands at p * sp + q * sq: p counts the longer
+// side, q the shorter one. WIDE: sp is 1, otherwise sq is.
+template <class T, bool WIDE>
+struct Panel {
+  const T* x;
+  long length, ld;
+  int n;
+  __device__ __forceinline__ float at(long p, int q) const {
+    return p < length && q < n ? (float)x[WIDE ? q * ld + p : p * ld + q]
+                               : 0.0f;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// G = X X^T in 64 bits, the upper tiles of it, for n <= 16 NT.
+// A wave takes 16 positions of the longer side at a time and has all tiles in
+// registers; the workgroup's waves are added up in order, and so are the
+// workgroups (gram_join_k): the same bits on every run.
+// ---------------------------------------------------------------------------
+//
+// 8 waves, or 4 from 7 tiles a side on: their 28 and 36 tiles need more than
+// the 256 registers that a wave of 8 can have.
+// ---------------------------------------------------------------------------
+__host__ __device__ constexpr int gram_waves(int nt) {
+  return nt < 7 ? 8 : 4;
+}
+
+template <class T, int NT, bool WIDE>
+__global__ __launch_bounds__(gram_waves(NT) * 64) void gram_k(
+    const T* __restrict__ x, long length, int n, long ld, long batch_x,
+    double* __restrict__ slab) {
+  constexpr int TILES = NT * (NT + 1) / 2, WAVES = gram_waves(NT);
+  __shared__ double sum[TILES * 256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = lane & 15, h = lane >> 4;
+  const Panel<T, WIDE> panel = {x + blockIdx.y * batch_x, length, ld, n};
+  v4d acc[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) acc[t] = v4d{0, 0, 0, 0};
+  const long groups = (length + 15) / 16;
+  const long stride = (long)gridDim.x * WAVES;
+  long g = (long)blockIdx.x * WAVES + wave;
+  float now[4][NT], next[4][NT];
+  auto load = [&](long g, float (&v)[4][NT]) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int q = i * 16 + c;
+      if (WIDE) {
+        // the sum over the longer side may take it in any order: four
+        // positions side by side for a lane
+        const long p = g * 16 + h * 4;
+        if (p + 4 <= length && q < n) {
+          const auto raw =
+              *(const typename Four<T>::Raw*)(panel.x + q * ld + p);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) v[t][i] = (float)raw.v[t];
+        } else {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) v[t][i] = panel.at(p + t, q);
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          v[t][i] = panel.at(g * 16 + t * 4 + h, q);
+      }
+    }
+  };
+  if (g < groups) load(g, now);
+  for (; g < groups; g += stride) {
+    if (g + stride < groups) load(g + stride, next);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      double v[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) v[i] = (double)now[t][i];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = i; j < NT; ++j)
+          acc[upper(NT, i, j)] = mma64(v[i], v[j], acc[upper(NT, i, j)]);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) now[t][i] = next[t][i];
+  }
+  for (int w = 0; w < WAVES; ++w) {
+    if (wave == w) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          double* to = &sum[t * 256 + (4 * i + h) * 16 + c];
+          *to = w ? *to + acc[t][i] : acc[t][i];
+        }
+    }
+    __syncthreads();
+  }
+  double* out = slab + ((long)blockIdx.y * gridDim.x + blockIdx.x) *
+                           (TILES * 256);
+  for (int i = threadIdx.x; i < TILES * 256; i += WAVES * 64)
+    out[i] = sum[i];
+}
+
+__global__ __launch_bounds__(1024) void gram_join_k(
+    const double* __restrict__ slab, int parts, double* __restrict__ out) {
+  __shared__ double sum[4][256];
+  const int e = threadIdx.x & 255, s = threadIdx.x >> 8;
+  const long size = (long)gridDim.x * 256;
+  const double* p = slab + (long)blockIdx.y * parts * size +
+                    blockIdx.x * 256 + e;
+  double v = 0.0;
+#pragma unroll 8
+  for (int i = s; i < parts; i += 4) v += p[i * size];
+  sum[s][e] = v;
+  __syncthreads();
+  if (s == 0)
+    out[blockIdx.y * size + blockIdx.x * 256 + e] =
+        (sum[0][e] + sum[1][e]) + (sum[2][e] + sum[3][e]);
+}
+
+// ---------------------------------------------------------------------------
+// Q from G_0, one workgroup for a matrix. All matrices are polynomials in
+// G_0: symmetric, and in any order under products, so only upper tiles are
+// held and computed. Two of them fit in LDS at n = 128; what else is alive
+// (Q, and a product on its way) stays in the registers of the waves whose
+// tiles they are.
+// ---------------------------------------------------------------------------
+constexpr int kFactorWaves = 8;
+
+template <int NT>
+__global__ __launch_bounds__(kFactorWaves * 64) void factor_k(
+    const double* __restrict__ gram, int n, int steps, double a, double b,
+    double c, double* __restrict__ out) {
+  constexpr int TILES = NT * (NT + 1) / 2;
+  constexpr int MINE = (TILES + kFactorWaves - 1) / kFactorWaves;
+  constexpr int LD = 17, SIZE = 16 * LD;  // rows of 17: no bank conflicts
+  __shared__ double s0[TILES * SIZE];
+  __shared__ double s1[TILES * SIZE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = lane & 15, h = lane >> 4;
+  gram += (long)blockIdx.x * TILES * 256;
+  out += (long)blockIdx.x * (16 * NT) * (16 * NT);
+  for (int i = threadIdx.x; i < TILES * 256; i += kFactorWaves * 64)
+    s0[(i >> 8) * SIZE + ((i >> 4) & 15) * LD + (i & 15)] = gram[i];
+  __syncthreads();
+  double trace = 0.0;
+  for (int k = lane; k < n; k += 64)
+    trace += s0[upper(NT, k >> 4, k >> 4) * SIZE + (k & 15) * (LD + 1)];
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) trace += __shfl_xor(trace, d);
+  __syncthreads();
+  // a matrix of zeros stays one; one that holds NaN or an infinity becomes
+  // NaN throughout
+  const bool fine = trace < INFINITY;
+  const double shrink = trace > 0.0 ? 1.0 / trace : 0.0;
+  for (int i = threadIdx.x; i < TILES * SIZE; i += kFactorWaves * 64)
+    s0[i] = fine ? s0[i] * shrink : 0.0;
+  __syncthreads();
+
+  int ti[MINE], tj[MINE];
+#pragma unroll
+  for (int t = 0; t < MINE; ++t) {
+    int k = wave + t * kFactorWaves, i = 0;
+    if (k >= TILES) k = TILES - 1;  // computed twice, stored once
+    while (i + 1 < NT && upper(NT, i + 1, i + 1) <= k) ++i;
+    ti[t] = i;
+    tj[t] = i + k - upper(NT, i, i);
+  }
+  auto mine = [&](int t) { return wave + t * kFactorWaves < TILES; };
+  auto product = [&](const double* u, const double* v, v4d (&r)[MINE]) {
+#pragma unroll
+    for (int t = 0; t < MINE; ++t) {
+      r[t] = v4d{0, 0, 0, 0};
+      if (!mine(t)) continue;
+      for (int k = 0; k < NT; ++k) {
+        const bool ua = ti[t] <= k, vb = k <= tj[t];
+        const double* pu = u + (ua ? upper(NT, ti[t], k)
+                                   : upper(NT, k, ti[t])) * SIZE +
+                           (ua ? col * LD + h : h * LD + col);
+        const double* pv = v + (vb ? upper(NT, k, tj[t])
+                                   : upper(NT, tj[t], k)) * SIZE +
+                           (vb ? h * LD + col : col * LD + h);
+        const int su = ua ? 4 : 4 * LD, sv = vb ? 4 * LD : 4;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          r[t] = mma64(pu[kk * su], pv[kk * sv], r[t]);
+      }
+    }
+  };
+  auto put = [&](double* s, const v4d (&r)[MINE]) {
+#pragma unroll
+    for (int t = 0; t < MINE; ++t)
+      if (mine(t))
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[upper(NT, ti[t], tj[t]) * SIZE + (4 * i + h) * LD + col] =
+              r[t][i];
+  };
+
+  v4d q[MINE], r[MINE], u[MINE];
+  for (int step = 0; step < steps; ++step) {
+    product(s0, s0, r);
+#pragma unroll
+    for (int t = 0; t < MINE; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const double g =
+            s0[upper(NT, ti[t], tj[t]) * SIZE + (4 * i + h) * LD + col];
+        const bool one = ti[t] == tj[t] && 4 * i + h == col;
+        r[t][i] = (one ? a : 0.0) + b * g + c * r[t][i];
+      }
+    put(s1, r);  // P
+    const bool more = step + 1 < steps;
+    if (step == 0) {
+#pragma unroll
+      for (int t = 0; t < MINE; ++t) q[t] = r[t];
+    }
+    __syncthreads();
+    if (more) product(s0, s1, u);  // G P
+    if (step > 0) {
+      __syncthreads();
+      put(s0, q);
+      __syncthreads();
+      product(s0, s1, q);
+    }
+    if (more) {
+      __syncthreads();
+      put(s0, u);
+      __syncthreads();
+      product(s0, s1, r);  // G P P
+      __syncthreads();
+      put(s0, r);
+      __syncthreads();
+    }
+  }
+  const double scale = !fine ? (double)NAN
+                             : trace > 0.0 ? 1.0 / sqrt(trace) : 0.0;
+#pragma unroll
+  for (int t = 0; t < MINE; ++t)
+    if (mine(t))
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int y = ti[t] * 16 + 4 * i + h, z = tj[t] * 16 + col;
+        const double v = q[t][i] * scale;
+        out[y * (16 * NT) + z] = v;
+        out[z * (16 * NT) + y] = v;
+      }
+}
+
+// ---------------------------------------------------------------------------
+// Out = Q X, 16 positions of the longer side for a wave at a time. Q lies in
+// LDS in the order in which the matrix instruction takes it. The k of an
+// instruction are chosen so that a lane's four of them stand side by side in
+// a tall panel: 16 s + 4 (lane / 16) + t.
+// ---------------------------------------------------------------------------
+template <class T, int NT, bool WIDE>
+__global__ __launch_bounds__(256) void apply_k(
+    const T* __restrict__ x, long length, int n, long ld, long batch_x,
+    const double* __restrict__ factor, T* __restrict__ out, long ld_out,
+    long batch_out) {
+  constexpr int N = 16 * NT;
+  __shared__ double qs[N * N];
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int c = lane & 15, h = lane >> 4;
+  factor += (long)blockIdx.y * N * N;
+  for (int i = threadIdx.x; i < N * N; i += 256) {
+    const int l = i & 63, j = (i >> 6) % NT, st = (i >> 6) / NT;
+    const int k = (st >> 2) * 16 + (l >> 4) * 4 + (st & 3);
+    qs[i] = factor[k * N + j * 16 + (l & 15)];
+  }
+  __syncthreads();
+  const Panel<T, WIDE> panel = {x + blockIdx.y * batch_x, length, ld, n};
+  out += blockIdx.y * batch_out;
+  const long groups = (length + 15) / 16;
+  const long stride = (long)gridDim.x * 4;
+  for (long g = (long)blockIdx.x * 4 + wave; g < groups; g += stride) {
+    const long p = g * 16 + c;
+    float v[NT][4];
+#pragma unroll
+    for (int s = 0; s < NT; ++s) {
+      const int q = s * 16 + h * 4;
+      if (!WIDE && p < length && q + 4 <= n) {
+        const auto raw = *(const typename Four<T>::Raw*)(panel.x + p * ld + q);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[s][t] = (float)raw.v[t];
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[s][t] = panel.at(p, q + t);
+      }
+    }
+    v4d acc[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j] = v4d{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < NT; ++s)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const double w = (double)v[s][t];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const double f = qs[((s * 4 + t) * NT + j) * 64 + lane];
+          acc[j] = WIDE ? mma64(f, w, acc[j]) : mma64(w, f, acc[j]);
+        }
+      }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const T y = (T)(float)acc[j][i];
+        if (WIDE) {
+          const int q = j * 16 + 4 * i + h;
+          if (q < n && p < length) out[q * ld_out + p] = y;
+        } else {
+          const long r = g * 16 + 4 * i + h;
+          const int q = j * 16 + c;
+          if (q < n && r < length) out[r * ld_out + q] = y;
+        }
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// n > 128
+// ---------------------------------------------------------------------------
+
+// sum of squares in 64 bits, one value for each workgroup
+template <class T>
+__global__ __launch_bounds__(256) void squares_k(
+    const T* __restrict__ x, int rows, int cols, long ld, long batch_x,
+    double* __restrict__ part) {
+  __shared__ double sum[4];
+  x += blockIdx.y * batch_x;
+  double v = 0.0;
+  for (int r = blockIdx.x; r < rows; r += gridDim.x)
+    for (int k = threadIdx.x; k < cols; k += 256) {
+      const double e = (double)(float)x[r * ld + k];
+      v += e * e;
+    }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    part[(long)blockIdx.y * gridDim.x + blockIdx.x] =
+        (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// X as fp16 numbers of magnitude up to 2^14, along both sides: [n][ld_d] and
+// [m][ld_t], filled up with zeros. X_0 = 2^-14 factor * what is stored; the
+// power of two in between is exact, the factor goes into the first step.
+template <class T>
+__global__ __launch_bounds__(256) void split_k(
+    const T* __restrict__ x, int rows, int cols, long ld, long batch_x,
+    int tall, const double* __restrict__ part, int parts, Halves d, Halves t,
+    float* __restrict__ factor) {
+  __shared__ float tile[64][65];
+  __shared__ double sum[4];
+  const int lane = threadIdx.x & 63;
+  double v = 0.0;
+  for (int i = threadIdx.x; i < parts; i += 256)
+    v += part[(long)blockIdx.y * parts + i];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  if (lane == 0) sum[threadIdx.x >> 6] = v;
+  __syncthreads();
+  const double norm = sqrt((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  const bool fine = norm < INFINITY;
+  int e = 0;
+  const double frac = fine ? frexp(norm, &e) : 0.0;  // norm = frac 2^e
+  if (blockIdx.x == 0 && threadIdx.x == 0)
+    factor[blockIdx.y] =
+        !fine ? NAN : norm > 0.0 ? (float)(1.0 / frac) : 0.0f;
+  x += blockIdx.y * batch_x;
+  // the tile in the input's own layout
+  const int across_tiles = (cols + 63) / 64;
+  const int r0 = blockIdx.x / across_tiles * 64;
+  const int c0 = blockIdx.x % across_tiles * 64;
+  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+    const int r = r0 + (i >> 6), k = c0 + (i & 63);
+    const float y = r < rows && k < cols ? (float)x[r * ld + k] : 0.0f;
+    tile[i >> 6][i & 63] = fine ? ldexpf(y, 14 - e) : 0.0f;
+  }
+  __syncthreads();
+  const Halves along = tall ? t : d, across = tall ? d : t;
+  for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+    const int r = i >> 4, k = (i & 15) * 4;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const Halves& o = w ? across : along;
+      const int row = (w ? c0 : r0) + r, at = (w ? r0 : c0) + k;
+      if (row >= (w ? cols : rows) || at >= o.ld) continue;
+      v4h hi, lo;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float y = w ? tile[k + u][r] : tile[r][k + u];
+        hi[u] = (_Float16)y;
+        lo[u] = (_Float16)(y - (float)hi[u]);
+      }
+      const long to = blockIdx.y * o.batch + (long)row * o.ld + at;
+      *(v4h*)(o.hi + to) = hi;
+      if (o.lo) *(v4h*)(o.lo + to) = lo;
+    }
+  }
+}
+
+// One product of a step, C = A B^T by tiles, then
+//   v = (alpha C + beta E) factor^power
+// either as halves, along both sides (for a symmetric result both are the
+// same matrix, and only its lower tiles are computed), or in the type of the
+// result.
+enum { kHalves, kFloat, kFp16, kBf16 };
+
+template <int OUT, int BM, int WM>
+__global__ __launch_bounds__((BM / WM) * (BM / WM) * 64) void step_k(
+    Sources s, Step p) {
+  typedef Tile<v4f, BM, BM, WM, WM> P;
+  __shared__ __attribute__((aligned(16))) char lds[P::kLds];
+  int ti, tj;
+  const int b = xcd_contiguous(blockIdx.x, gridDim.x);
+  if (p.symmetric) triangle(b, ti, tj);
+  else banded(b, p.tm, p.tn, ti, tj);
+  v4f acc[P::MI][P::NJ];
+  const long z = blockIdx.y;
+  P::run(s, ti * BM, tj * BM, z, 0,
+         s.parts * ((s.kbytes + kStep - 1) / kStep), lds, acc);
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int wm0 = ti * BM + wave / (BM / WM) * WM;
+  const int wn0 = tj * BM + wave % (BM / WM) * WM;
+  const int c = lane & 15, h = lane >> 4;
+  const int rows = s.rows_a, cols = s.rows_b;
+  float alpha = p.alpha, beta = p.beta;
+  if (p.power) {
+    const float f = p.power == 2 ? p.factor[z] * p.factor[z] : p.factor[z];
+    alpha *= f;
+    beta *= f;
+  }
+  // the wave's own piece of LDS: 16 columns of its part, for storing along
+  // the other side
+  constexpr int LD = WM + 8;
+  _Float16* th = (_Float16*)lds + wave * (2 * 16 * LD);
+  _Float16* tl = th + 16 * LD;
+  const bool across = OUT == kHalves && p.t.hi && !(p.symmetric && ti == tj);
+#pragma unroll
+  for (int j = 0; j < P::NJ; ++j) {
+    const int n = wn0 + j * 16 + h * 4;
+#pragma unroll
+    for (int i = 0; i < P::MI; ++i) {
+      const int m = wm0 + i * 16 + c;
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = alpha * acc[i][j][r];
+      if (p.e.hi && m < rows && n < cols) {
+        const long at = z * p.e.batch + (long)m * p.e.ld + n;
+        const v4h eh = *(const v4h*)(p.e.hi + at);
+        v4h el = {0, 0, 0, 0};
+        if (p.e.lo) el = *(const v4h*)(p.e.lo + at);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          v[r] += beta * ((float)eh[r] + (float)el[r]);
+      }
+      if (OUT == kHalves) {
+        v4h hi, lo;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          // rows and columns that are not there count as zeros later
+          if (m >= rows || n + r >= cols) v[r] = 0.0f;
+          hi[r] = (_Float16)v[r];
+          lo[r] = (_Float16)(v[r] - (float)hi[r]);
+        }
+        if (p.d.hi && m < rows && n < p.d.ld) {
+          const long at = z * p.d.batch + (long)m * p.d.ld + n;
+          *(v4h*)(p.d.hi + at) = hi;
+          if (p.d.lo) *(v4h*)(p.d.lo + at) = lo;
+        }
+        if (across) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            th[(h * 4 + r) * LD + i * 16 + c] = hi[r];
+            tl[(h * 4 + r) * LD + i * 16 + c] = lo[r];
+          }
+        }
+      } else if (m < rows) {
+        const long step = p.tall ? p.ld_out : 1;
+        const long at = z * p.batch_out +
+                        (p.tall ? n * p.ld_out + m : m * p.ld_out + n);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < cols) {
+            if (OUT == kFloat) ((float*)p.out)[at + r * step] = v[r];
+            else if (OUT == kFp16)
+              ((_Float16*)p.out)[at + r * step] = (_Float16)v[r];
+            else ((__bf16*)p.out)[at + r * step] = (__bf16)v[r];
+          }
+      }
+    }
+    if (across) {
+      // a wave's own writes and reads of LDS go in order; the compiler has to
+      // keep them so
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int u = 0; u < 16 * (WM / 8) / 64; ++u) {
+        const int k = u * 64 + lane;
+        const int row = k / (WM / 8), m = wm0 + k % (WM / 8) * 8;
+        const int nn = wn0 + j * 16 + row;
+        if (nn < cols && m < p.t.ld) {
+          const long at = z * p.t.batch + (long)nn * p.t.ld + m;
+          *(v8h*)(p.t.hi + at) = *(const v8h*)(th + row * LD + m - wm0);
+          if (p.t.lo)
+            *(v8h*)(p.t.lo + at) = *(const v8h*)(tl + row * LD + m - wm0);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  }
+}
+
+template <int OUT>
+void step_as(Sources s, Step p, int batch, hipStream_t st) {
+  // 128 x 128 tiles once they fill the chip, 64 x 64 ones below
+  const long m128 = (s.rows_a + 127) / 128, n128 = (s.rows_b + 127) / 128;
+  const long count = (p.symmetric ? m128 * (m128 + 1) / 2 : m128 * n128);
+  const int size = count * batch >= 256 ? 128 : 64;
+  p.tm = (s.rows_a + size - 1) / size;
+  p.tn = (s.rows_b + size - 1) / size;
+  const dim3 grid(p.symmetric ? p.tm * (p.tm + 1) / 2 : p.tm * p.tn, batch);
+  if (size == 128)
+    hipLaunchKernelGGL((step_k<OUT, 128, 64>), grid, dim3(256), 0, st, s, p);
+  else
+    hipLaunchKernelGGL((step_k<OUT, 64, 32>), grid, dim3(256), 0, st, s, p);
+}
+
+template <class T, int NT>
+void gram_as(const T* x, bool wide, long length, int n, long ld, long bx,
+             int batch, double* slab, int parts, hipStream_t st) {
+  const dim3 grid(parts, batch), block(gram_waves(NT) * 64);
+  if (wide)
+    hipLaunchKernelGGL((gram_k<T, NT, true>), grid, block, 0, st, x, length,
+                       n, ld, bx, slab);
+  else
+    hipLaunchKernelGGL((gram_k<T, NT, false>), grid, block, 0, st, x, length,
+                       n, ld, bx, slab);
+}
+
+template <class T, int NT>
+void apply_as(const T* x, bool wide, long length, int n, long ld, long bx,
+              int batch, const double* factor, T* out, long ld_out,
+              long batch_out, int blocks, hipStream_t st) {
+  const dim3 grid(blocks, batch), block(256);
+  if (wide)
+    hipLaunchKernelGGL((apply_k<T, NT, true>), grid, block, 0, st, x, length,
+                       n, ld, bx, factor, out, ld_out, batch_out);
+  else
+    hipLaunchKernelGGL((apply_k<T, NT, false>), grid, block, 0, st, x, length,
+                       n, ld, bx, factor, out, ld_out, batch_out);
+}
+
+#define BY_TILES(nt, CALL) \
+  switch (nt) {            \
+    case 1: CALL(1) break; \
+    case 2: CALL(2) break; \
+    case 3: CALL(3) break; \
+    case 4: CALL(4) break; \
+    case 5: CALL(5) break; \
+    case 6: CALL(6) break; \
+    case 7: CALL(7) break; \
+    default: CALL(8)       \
+  }
+
+template <class T>
+void gram_type(const T* x, bool wide, long length, int n, long ld, long bx,
+               int batch, double* slab, int parts, hipStream_t st) {
+#define CALL(NT) \
+  gram_as<T, NT>(x, wide, length, n, ld, bx, batch, slab, parts, st);
+  BY_TILES((n + 15) / 16, CALL)
+#undef CALL
+}
+
+template <class T>
+void apply_type(const T* x, bool wide, long length, int n, long ld, long bx,
+                int batch, const double* factor, T* out, long ld_out,
+                long batch_out, int blocks, hipStream_t st) {
+#define CALL(NT)                                                           \
+  apply_as<T, NT>(x, wide, length, n, ld, bx, batch, factor, out, ld_out, \
+                  batch_out, blocks, st);
+  BY_TILES((n + 15) / 16, CALL)
+#undef CALL
+}
+
+}  // namespace
+
+#define BY_TYPE(dtype, CALL)             \
+  if (dtype == 0) { CALL(float) }        \
+  else if (dtype == 1) { CALL(_Float16) } \
+  else { CALL(__bf16) }
+
+extern "C" int gram_parts(long length, int n, int batch) {
+  const long groups = (length + 15) / 16;
+  const long each = 4 * gram_waves((n + 15) / 16);  // 4 groups for a wave
+  const long parts = (groups + each - 1) / each;
+  const long most = batch < 256 ? 256 / batch : 1;
+  return (int)(parts < 1 ? 1 : parts > most ? most : parts);
+}
+
+extern "C" void launch_gram(const void* x, int dtype, int wide, long length,
+                            int n, long ld, long batch_x, int batch,
+                            double* slab, int parts, double* gram,
+                            hipStream_t st) {
+#define CALL(T)                                                         \
+  gram_type((const T*)x, wide, length, n, ld, batch_x, batch,           \
+            parts > 1 ? slab : gram, parts, st);
+  BY_TYPE(dtype, CALL)
+#undef CALL
+  const int nt = (n + 15) / 16;
+  if (parts > 1)
+    hipLaunchKernelGGL(gram_join_k, dim3(nt * (nt + 1) / 2, batch),
+                       dim3(1024), 0, st, slab, parts, gram);
+}
+
+extern "C" void launch_factor(const double* gram, int n, int steps, double a,
+                              double b, double c, int batch, double* factor,
+                              hipStream_t st) {
+#define CALL(NT)                                                         \
+  hipLaunchKernelGGL((factor_k<NT>), dim3(batch), dim3(kFactorWaves * 64), \
+                     0, st, gram, n, steps, a, b, c, factor);
+  BY_TILES((n + 15) / 16, CALL)
+#undef CALL
+}
+
+extern "C" void launch_apply(const void* x, int dtype, int wide, long length,
+                             int n, long ld, long batch_x, int batch,
+                             const double* factor, void* out, long ld_out,
+                             long batch_out, hipStream_t st) {
+  const long groups = (length + 15) / 16;
+  const long want = (groups + 15) / 16;
+  const long most = n <= 64 ? 1024 : 256;
+  const int blocks = (int)(want < 1 ? 1 : want > most ? most : want);
+#define CALL(T)                                                           \
+  apply_type((const T*)x, wide, length, n, ld, batch_x, batch, factor,    \
+             (T*)out, ld_out, batch_out, blocks, st);
+  BY_TYPE(dtype, CALL)
+#undef CALL
+}
+
+extern "C" void launch_split(const void* x, int dtype, int rows, int cols,
+                             long ld, long batch_x, int batch, double* part,
+                             int parts, Halves d, Halves t, float* factor,
+                             hipStream_t st) {
+  const int tall = rows > cols;
+  const dim3 grid(((cols + 63) / 64) * ((rows + 63) / 64), batch);
+#define CALL(T)                                                             \
+  hipLaunchKernelGGL((squares_k<T>), dim3(parts, batch), dim3(256), 0, st,  \
+                     (const T*)x, rows, cols, ld, batch_x, part);           \
+  hipLaunchKernelGGL((split_k<T>), grid, dim3(256), 0, st, (const T*)x,     \
+                     rows, cols, ld, batch_x, tall, part, parts, d, t,      \
+                     factor);
+  BY_TYPE(dtype, CALL)
+#undef CALL
+}
+
+// a, b: the operands' hi and lo; parts 1: hi hi, 2: hi hi + hi lo, 3: all.
+extern "C" void launch_step(Halves a, int rows_a, Halves b, int rows_b, int k,
+                            int parts, Step p, int batch, int out,
+                            hipStream_t st) {
+  Sources s = {};
+  s.a[0] = (const char*)a.hi;
+  s.b[0] = (const char*)b.hi;
+  s.a[1] = (const char*)a.hi;
+  s.b[1] = (const char*)b.lo;
+  s.a[2] = (const char*)a.lo;
+  s.b[2] = (const char*)b.hi;
+  s.batch_a = a.batch * 2;
+  s.batch_b = b.batch * 2;
+  s.row_a = (unsigned)(a.ld * 2);
+  s.row_b = (unsigned)(b.ld * 2);
+  s.rows_a = rows_a;
+  s.rows_b = rows_b;
+  s.kbytes = (k + 63) / 64 * 128;  // the filling is zeros
+  s.parts = parts;
+  switch (out) {
+    case kHalves: step_as<kHalves>(s, p, batch, st); break;
+    case kFloat: step_as<kFloat>(s, p, batch, st); break;
+    case kFp16: step_as<kFp16>(s, p, batch, st); break;
+    default: step_as<kBf16>(s, p, batch, st);
+  }
+}

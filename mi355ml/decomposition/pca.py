@@ -4,6 +4,10 @@ Mean-center (fused column-stats pass + one small allreduce) then SVD:
 svd_solver 'full'/'tsqr' -> distributed TSQR (ops/linalg.tsqr, SURVEY A.1);
 'randomized' -> Halko range finder (ops/linalg.svd_compressed);
 'auto' -> randomized when n_components < 0.8·ncols, else tsqr.
+
+power_iteration_normalizer ("QR" or "newton_schulz") is what the range finder
+keeps its panel's columns apart with; transform_dtype ("float32" or "int8")
+what transform computes its product in.
 """
 
 from __future__ import annotations
@@ -16,17 +20,22 @@ from ..base import BaseEstimator, TransformerMixin, check_array, check_is_fitted
 from ..core.array import DistArray
 from ..ops import affine_transform
 from ..ops.linalg import svd_compressed, tsqr
+from ._project import check_transform_dtype, project
 
 
 class PCA(BaseEstimator, TransformerMixin):
     def __init__(self, n_components: Optional[int] = None,
                  whiten: bool = False, svd_solver: str = "auto",
-                 iterated_power: int = 2, random_state: int = 0):
+                 iterated_power: int = 2, random_state: int = 0,
+                 power_iteration_normalizer: str = "QR",
+                 transform_dtype: str = "float32"):
         self.n_components = n_components
         self.whiten = whiten
         self.svd_solver = svd_solver
         self.iterated_power = iterated_power
         self.random_state = random_state
+        self.power_iteration_normalizer = power_iteration_normalizer
+        self.transform_dtype = transform_dtype
 
     def _solver(self, d: int, k: int) -> str:
         if self.svd_solver != "auto":
@@ -53,7 +62,8 @@ class PCA(BaseEstimator, TransformerMixin):
         elif solver == "randomized":
             U, s, Vh = svd_compressed(
                 Xc, k, n_power_iter=self.iterated_power,
-                seed=int(self.random_state or 0), compute_u=need_u)
+                seed=int(self.random_state or 0), compute_u=need_u,
+                normalizer=self.power_iteration_normalizer)
             Uk = U
         else:
             raise ValueError(f"unknown svd_solver {solver!r}")
@@ -130,6 +140,7 @@ class PCA(BaseEstimator, TransformerMixin):
 
     def transform(self, X):
         check_is_fitted(self, "components_")
+        check_transform_dtype(self.transform_dtype)
         X = check_array(X, col_ok=True)
         V = self.components_.to(X.device)
         mean = self.mean_.to(X.device)
@@ -138,22 +149,18 @@ class PCA(BaseEstimator, TransformerMixin):
             # feature-parallel: Σ_r (X_loc - μ_loc) V_locᵀ → one [m, k]
             # allreduce
             lo, hi = X.col_offset, X.col_offset + X.local_cols
-            z = (X.local - mean[lo:hi][None, :]) @ V[:, lo:hi].to(X.dtype).t()
+            z = project(X.local - mean[lo:hi][None, :], V[:, lo:hi],
+                        self.transform_dtype)
             if X.comm.world_size > 1:
                 X.comm.all_reduce(z)
             if self.whiten:
                 z = z * (1.0 / self.explained_variance_.to(
                     z.device).sqrt()).to(z.dtype)
             return Replicated(z, X.comm)
-        if self.whiten:
-            inv = (1.0 / self.explained_variance_.to(X.device).sqrt())
-
-            def _t(t):
-                return ((t - mean) @ V.to(t.dtype).t()) * inv.to(t.dtype)
-        else:
-            def _t(t):
-                return (t - mean) @ V.to(t.dtype).t()
-        return X.map_local(_t)
+        inv = (1.0 / self.explained_variance_.to(X.device).sqrt()
+               if self.whiten else None)
+        return X.map_local(
+            lambda t: project(t - mean, V, self.transform_dtype, inv))
 
     def inverse_transform(self, X):
         check_is_fitted(self, "components_")

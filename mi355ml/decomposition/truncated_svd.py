@@ -1,7 +1,9 @@
 """TruncatedSVD (dask_ml/decomposition/truncated_svd.py parity).
 
 Same machinery as PCA without centering; algorithm 'tsqr' (exact) or
-'randomized' (range finder).
+'randomized' (range finder, whose panel is kept apart by
+power_iteration_normalizer "QR" or "newton_schulz"). transform_dtype
+("float32" or "int8") is what transform computes its product in.
 """
 
 from __future__ import annotations
@@ -11,15 +13,20 @@ import torch
 from ..base import BaseEstimator, TransformerMixin, check_array, check_is_fitted
 from ..core.array import DistArray
 from ..ops.linalg import svd_compressed, tsqr
+from ._project import check_transform_dtype, project
 
 
 class TruncatedSVD(BaseEstimator, TransformerMixin):
     def __init__(self, n_components: int = 2, algorithm: str = "tsqr",
-                 n_iter: int = 5, random_state: int = 0, tol: float = 0.0):
+                 n_iter: int = 5, random_state: int = 0, tol: float = 0.0,
+                 power_iteration_normalizer: str = "QR",
+                 transform_dtype: str = "float32"):
         self.n_components = n_components
         self.algorithm = algorithm
         self.n_iter = n_iter
         self.random_state = random_state
+        self.power_iteration_normalizer = power_iteration_normalizer
+        self.transform_dtype = transform_dtype
         self.tol = tol
 
     def _fit(self, X: DistArray, need_u: bool = False):
@@ -54,7 +61,9 @@ class TruncatedSVD(BaseEstimator, TransformerMixin):
         elif self.algorithm == "randomized":
             U, s, Vh = svd_compressed(X, k, n_power_iter=self.n_iter,
                                       seed=int(self.random_state or 0),
-                                      compute_u=need_u)
+                                      compute_u=need_u,
+                                      normalizer=self
+                                      .power_iteration_normalizer)
         else:
             raise ValueError(f"unknown algorithm {self.algorithm!r}")
         n = float(X.global_rows)
@@ -80,17 +89,18 @@ class TruncatedSVD(BaseEstimator, TransformerMixin):
 
     def transform(self, X):
         check_is_fitted(self, "components_")
+        check_transform_dtype(self.transform_dtype)
         X = check_array(X, col_ok=True)
         V = self.components_.to(X.device)
         from ..core.colarray import ColDistArray, Replicated
         if isinstance(X, ColDistArray):
             # Σ_r X_loc V_locᵀ → one [m, k] allreduce
             vl = V[:, X.col_offset:X.col_offset + X.local_cols]
-            z = X.local @ vl.to(X.dtype).t()
+            z = project(X.local, vl, self.transform_dtype)
             if X.comm.world_size > 1:
                 X.comm.all_reduce(z)
             return Replicated(z, X.comm)
-        return X.map_local(lambda t: t @ V.to(t.dtype).t())
+        return X.map_local(lambda t: project(t, V, self.transform_dtype))
 
     def inverse_transform(self, X):
         check_is_fitted(self, "components_")

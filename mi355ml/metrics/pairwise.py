@@ -11,7 +11,7 @@ import torch
 
 from ..base import check_array
 from ..core.array import DistArray
-from ..ops import closest_center
+from ..ops import closest_center, int8_linear, quantize_rows
 
 
 def euclidean_distances(X, Y: torch.Tensor, squared: bool = False) -> DistArray:
@@ -65,9 +65,17 @@ def pairwise_distances(X, Y: torch.Tensor, metric: str = "euclidean"):
     return Xd.map_local(_block)
 
 
-def linear_kernel(X, Y: torch.Tensor):
+def linear_kernel(X, Y: torch.Tensor, dtype: str = "float32"):
+    """Inner products of X's rows with those of a small replicated Y; dtype
+    "int8" takes them of 8-bit rows with a scale each."""
+    if dtype not in ("float32", "int8"):
+        raise ValueError(f"unknown dtype {dtype!r}; choose float32 or int8")
     Xd = check_array(X)
     Y = torch.as_tensor(Y, dtype=Xd.dtype, device=Xd.device)
+    if dtype == "int8":
+        yq, ys = quantize_rows(Y.float())
+        return Xd.map_local(
+            lambda t: int8_linear(t.float(), yq, ys).to(t.dtype))
     return Xd.map_local(lambda t: t @ Y.t())
 
 

@@ -20,6 +20,7 @@ from .glm import glm_value_grad
 from .kmeans import kmeans_assign, closest_center
 from .elementwise import affine_transform
 from .int8 import int8_linear, int8_matmul, quantize_rows
+from .orthogonalize import newton_schulz
 
 __all__ = [
     "col_moments",
@@ -32,5 +33,6 @@ __all__ = [
     "affine_transform",
     "int8_linear",
     "int8_matmul",
+    "newton_schulz",
     "quantize_rows",
 ]

@@ -25,6 +25,9 @@ import torch
 
 from ..core.array import DistArray
 from ..core import random as mlrand
+from ._ext import hip_ext, use_hip
+from .orthogonalize import (COEFFICIENTS, MAX_PANEL, check_iteration,
+                            factor_of_gram)
 
 
 def _block_rows_for(d: int) -> int:
@@ -150,10 +153,49 @@ def tsqr(X: DistArray, compute_svd: bool = False, compute_q: bool = True):
             s.to(X.dtype), vh.to(X.dtype))
 
 
+def newton_schulz_panel(X: DistArray, steps: int = 5,
+                        coefficients=COEFFICIENTS) -> DistArray:
+    """A tall row-sharded panel orthogonalised by Newton-Schulz products.
+
+    The same iteration as ``ops.newton_schulz``, taken on the panel's Gram
+    matrix: one pass over the shard for its part of it (in 64 bits), ONE
+    all-reduce, the steps on [d, d] matrices on every rank, and one pass for
+    the product. No factorisation that could fail, and no wait for the
+    device: panels of any rank pass. At most 128 columns.
+    """
+    c = check_iteration(steps, coefficients)
+    a = X._as2d()
+    d = a.shape[1]
+    if not 1 <= d <= MAX_PANEL:
+        raise ValueError(f"a panel has 1 to {MAX_PANEL} columns, got {d}")
+    comm = X.comm
+    if use_hip(a):
+        gram = hip_ext().panel_gram(a)
+        if comm.world_size > 1:
+            comm.all_reduce(gram)
+        out = hip_ext().panel_finish(a, gram, int(steps), *c)
+    else:
+        ad = a.double()
+        gram = ad.t() @ ad
+        if comm.world_size > 1:
+            comm.all_reduce(gram)
+        out = (ad @ factor_of_gram(gram, int(steps), c)).to(a.dtype)
+    return DistArray(out, X.global_rows, X.row_offset, comm)
+
+
+#: what holds the panel of a power iteration apart between two products
+NORMALIZERS = ("QR", "newton_schulz")
+
+
 def svd_compressed(X: DistArray, k: int, n_power_iter: int = 2,
                    n_oversamples: int = 10, seed: int = 0,
-                   compute_u: bool = True):
+                   compute_u: bool = True, normalizer: str = "QR"):
     """Randomized truncated SVD (Halko/Martinsson/Tropp), f32 GEMMs.
+
+    normalizer: what keeps the panel's columns apart between the products of
+    the power iteration, "QR" (TSQR) or "newton_schulz" (cheaper, columns
+    only nearly orthonormal, at most 128 of them; the last panel is made
+    orthonormal by TSQR either way).
 
     Returns (U DistArray [m, k] or None, s [k], Vh [k, d]).
     """
@@ -161,17 +203,29 @@ def svd_compressed(X: DistArray, k: int, n_power_iter: int = 2,
     m, d = X.global_rows, a.shape[1]
     comm = X.comm
     ell = min(k + n_oversamples, d, m)
+    if normalizer not in NORMALIZERS:
+        raise ValueError(f"unknown normalizer {normalizer!r}; choose from "
+                         f"{NORMALIZERS}")
+    if normalizer == "newton_schulz" and ell > MAX_PANEL:
+        raise ValueError(f"newton_schulz takes panels of at most {MAX_PANEL} "
+                         f"columns, got {ell} (components and oversamples)")
+
+    def normalize(Y: DistArray, last: bool) -> DistArray:
+        if normalizer == "QR" or last:
+            return tsqr(Y)[0]
+        return newton_schulz_panel(Y)
+
     g = mlrand.generator(seed, shard_id=0xABCD, device=a.device)
     omega = torch.randn(d, ell, generator=g, device=a.device, dtype=X.dtype)
     Y = DistArray(a @ omega, m, X.row_offset, comm)
-    Q, _ = tsqr(Y)
-    for _ in range(n_power_iter):
+    Q = normalize(Y, last=n_power_iter == 0)
+    for i in range(n_power_iter):
         # Z = Xᵀ Q  (allreduce, C6), then re-orthogonalize X·Z
         z = a.t() @ Q._as2d()
         if comm.world_size > 1:
             comm.all_reduce(z)
         Y = DistArray(a @ z, m, X.row_offset, comm)
-        Q, _ = tsqr(Y)
+        Q = normalize(Y, last=i + 1 == n_power_iter)
     # B = Qᵀ X : [ell, d] via allreduce (f64 for the small final factor)
     b = (Q._as2d().t() @ a).to(torch.float64)
     if comm.world_size > 1:

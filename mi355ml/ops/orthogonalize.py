@@ -1,0 +1,94 @@
+"""Orthogonalising matrices by Newton-Schulz products.
+
+X_0 = X / ||X||_F, then ``steps`` times
+
+    X <- a X + (b G + c G^2) X,    G = X X^T (of the shorter side)
+
+which leaves the singular vectors and takes each singular value through
+s <- a s + b s^3 + c s^5: towards the nearest matrix with orthonormal rows
+(or columns), X (X^T X)^(-1/2), with products alone. The default coefficients
+raise small singular values fastest (by 3.4 a step) and bring them to between
+0.68 and 1.14 rather than to 1, which is what an update's direction (momentum
+orthogonalised before it is applied, a matrix at a time) or the panel of a
+power iteration needs; (1.875, -1.25, 0.375) converges to 1 for more steps.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Tuple
+
+import torch
+
+from ._ext import hip_ext, use_hip
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+#: most columns of a panel that is spread over ranks
+MAX_PANEL = 128
+
+
+def check_iteration(steps: int, coefficients) -> Tuple[float, float, float]:
+    if isinstance(steps, bool) or int(steps) != steps or \
+            not 1 <= steps <= 1000:
+        raise ValueError(f"steps must be a whole number from 1 to 1000, got "
+                         f"{steps!r}")
+    c = tuple(float(v) for v in coefficients)
+    if len(c) != 3 or not all(math.isfinite(v) for v in c):
+        raise ValueError(f"coefficients must be three finite numbers, got "
+                         f"{coefficients!r}")
+    return c
+
+
+def factor_of_gram(gram: torch.Tensor, steps: int, coefficients
+                   ) -> torch.Tensor:
+    """Q with X_steps = X Q, from gram = X^T X (float64, CPU form)."""
+    a, b, c = coefficients
+    trace = gram.diagonal(dim1=-2, dim2=-1).sum(-1)[..., None, None]
+    fine = torch.isfinite(trace)
+    some = fine & (trace > 0)
+    g = torch.where(some, gram / torch.where(some, trace, 1.0), 0.0)
+    eye = torch.eye(g.shape[-1], dtype=g.dtype, device=g.device)
+    q = eye.expand_as(g)
+    for _ in range(steps):
+        p = a * eye + b * g + c * (g @ g)
+        q = q @ p
+        g = p @ g @ p
+    q = torch.where(some, q / torch.where(some, trace, 1.0).sqrt(), 0.0)
+    return torch.where(fine, q, float("nan"))
+
+
+def newton_schulz(x: torch.Tensor, steps: int = 5,
+                  coefficients: Tuple[float, float, float] = COEFFICIENTS
+                  ) -> torch.Tensor:
+    """x [..., m, k] orthogonalised, each matrix of a batch for itself.
+
+    x: 2-D or 3-D, float32, float16 or bfloat16, of any shape and strides
+    (a matrix whose rows are not contiguous is copied first); returns a
+    contiguous tensor of the same shape and type. Products are summed in 32
+    bits or more. A matrix of zeros gives zeros; one that holds an infinity
+    or NaN gives NaN throughout. Not differentiable.
+    """
+    a, b, c = check_iteration(steps, coefficients)
+    if x.dim() not in (2, 3):
+        raise ValueError(f"x must be 2-D or 3-D, got {x.dim()}-D")
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"x must be float32, float16 or bfloat16, got "
+                        f"{x.dtype}")
+    if use_hip(x):
+        return hip_ext().newton_schulz(x.detach(), int(steps), a, b, c)
+    x = x.detach()
+    if x.numel() == 0:
+        return x.new_empty(x.shape)
+    y = x.double()
+    y = y.transpose(-2, -1) if y.shape[-2] > y.shape[-1] else y
+    norm = y.square().sum(dim=(-2, -1), keepdim=True).sqrt()
+    fine = torch.isfinite(norm)
+    some = fine & (norm > 0)
+    y = torch.where(some, y / torch.where(some, norm, 1.0), 0.0)
+    for _ in range(int(steps)):
+        g = y @ y.transpose(-2, -1)
+        y = a * y + (b * g + c * (g @ g)) @ y
+    y = torch.where(fine, y, float("nan"))
+    y = y.transpose(-2, -1) if x.shape[-2] > x.shape[-1] else y
+    return y.to(x.dtype).contiguous()

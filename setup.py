@@ -21,8 +21,11 @@ ext = CUDAExtension(
         "mi355ml/_hip/kernels.hip",
         "mi355ml/_hip/bindings_int8.cpp",
         "mi355ml/_hip/int8.hip",
+        "mi355ml/_hip/bindings_orthogonalize.cpp",
+        "mi355ml/_hip/orthogonalize.hip",
     ],
-    depends=["mi355ml/_hip/tile_product.h"],
+    depends=["mi355ml/_hip/orthogonalize.h",
+             "mi355ml/_hip/tile_product.h"],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
         # packed fp32 instructions are off: some of their forms have given

@@ -206,7 +206,89 @@ def test_refusals():
         ops.int8_linear(torch.ones(3, 3, dtype=torch.int32), q, s)
 
 
+def _check_estimators():
+    import numpy as np
+    from mi355ml.core.array import from_numpy
+    from mi355ml.decomposition import PCA, TruncatedSVD
+    from mi355ml.metrics.pairwise import linear_kernel
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((500, 5)) @ rng.standard_normal((5, 60)) + 2
+    x += rng.standard_normal((500, 60)) * 0.1
+    X = from_numpy(x.astype(np.float32))
+
+    def close(got, want):
+        got, want = got.gather().cpu(), want.gather().cpu()
+        assert got.shape == want.shape and got.dtype == want.dtype
+        # values of up to 4 times their row's root mean square are held within
+        # half a step of 127: 4 / 254 / sqrt(3) on either side, at most 1.3%
+        assert ((got - want).norm() / want.norm()) < 0.013
+        assert not torch.equal(got, want)
+
+    for make in (lambda t: PCA(5, transform_dtype=t),
+                 lambda t: PCA(5, whiten=True, transform_dtype=t),
+                 lambda t: TruncatedSVD(5, transform_dtype=t)):
+        close(make("int8").fit(X).transform(X),
+              make("float32").fit(X).transform(X))
+    Y = torch.as_tensor(x[:7].astype(np.float32))
+    close(linear_kernel(X, Y, dtype="int8"), linear_kernel(X, Y))
+    with pytest.raises(ValueError, match="transform_dtype"):
+        PCA(5, transform_dtype="int4").fit(X).transform(X)
+    with pytest.raises(ValueError, match="dtype"):
+        linear_kernel(X, Y, dtype="fp8")
+
+
+def test_estimators():
+    _check_estimators()
+
+
+def _col_transform(rank, world):
+    import numpy as np
+    from mi355ml.core.colarray import from_numpy_cols
+    from mi355ml.decomposition import TruncatedSVD
+    x = np.random.default_rng(0).standard_normal((40, 30)).astype(np.float32)
+    X = from_numpy_cols(x)
+    want = TruncatedSVD(3).fit(X)
+    z = want.transform(X).local
+    got = TruncatedSVD(3, transform_dtype="int8").fit(X).transform(X).local
+    assert ((got - z).norm() / z.norm()) < 0.02
+
+
+def test_columns_spread_over_ranks(mp_runner):
+    mp_runner(_col_transform, world=2)
+
+
 # ------------------------------------------------------------------ GPU
+
+@pytest.mark.gpu
+def test_gpu_estimators():
+    _check_estimators()
+
+
+@pytest.mark.gpu
+def test_gpu_panel_then_8_bit_projection():
+    """The operators as they are used together: a range finder that holds its
+    panel apart by Newton-Schulz products, then requests answered in 8 bits,
+    a batch and single rows of it."""
+    from mi355ml import datasets
+    from mi355ml.decomposition import TruncatedSVD
+    X, _ = datasets.make_classification(n_samples=20_000, n_features=100,
+                                        n_informative=10, random_state=0)
+    kw = dict(n_components=8, algorithm="randomized", n_iter=3,
+              random_state=0)
+    ref = TruncatedSVD(**kw).fit(X)
+    est = TruncatedSVD(power_iteration_normalizer="newton_schulz",
+                       transform_dtype="int8", **kw).fit(X)
+    torch.testing.assert_close(est.singular_values_, ref.singular_values_,
+                               rtol=1e-3, atol=0)
+    z = est.transform(X).local
+    want = X.local.double() @ est.components_.double().t()
+    # half a step of 127 on values of at most 5 times their row's root mean
+    # square, on either side
+    assert (z.double() - want).norm() / want.norm() < 0.02
+    for rows in (1, 3, 70):
+        part = type(X)(X.local[:rows].contiguous(), rows, 0, X.comm)
+        assert torch.equal(est.transform(part).local, z[:rows])
+
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", FLOATS)

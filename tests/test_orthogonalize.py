@@ -1,0 +1,354 @@
+"""Newton-Schulz orthogonalisation: the CPU form against singular values and
+the refusals here, the HIP kernels against 64-bit arithmetic with -m gpu."""
+
+import numpy as np
+import pytest
+import torch
+
+from mi355ml import ops
+from mi355ml.core.array import DistArray, from_numpy
+from mi355ml.decomposition import PCA, TruncatedSVD
+from mi355ml.ops.linalg import newton_schulz_panel, svd_compressed
+from mi355ml.ops.orthogonalize import COEFFICIENTS
+
+FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _matrix(*shape, dtype=torch.float32, seed=0, scale=1e-2):
+    """A few strong directions over noise, as a gradient has them."""
+    g = torch.Generator().manual_seed(seed)
+    *b, m, k = shape
+    r = min(8, m, k)
+    x = torch.randn(*shape, generator=g)
+    x += (torch.randn(*b, m, r, generator=g) * torch.logspace(0.5, -0.5, r)
+          ) @ torch.randn(*b, r, k, generator=g)
+    return (x * scale).to(dtype)
+
+
+def _by_singular_values(x, steps=5, c=COEFFICIENTS):
+    u, s, vh = torch.linalg.svd(x.double(), full_matrices=False)
+    s = s / s.square().sum(-1, keepdim=True).sqrt()
+    for _ in range(steps):
+        s = c[0] * s + c[1] * s ** 3 + c[2] * s ** 5
+    return (u * s[..., None, :]) @ vh
+
+
+def _iterate(x, dtype, steps=5, c=COEFFICIENTS):
+    y = x.to(dtype)
+    y = y.transpose(-2, -1) if y.shape[-2] > y.shape[-1] else y
+    y = y / x.double().square().sum((-2, -1), keepdim=True).sqrt().to(dtype)
+    for _ in range(steps):
+        g = y @ y.transpose(-2, -1)
+        y = c[0] * y + (c[1] * g + c[2] * (g @ g)) @ y
+    return y.transpose(-2, -1) if x.shape[-2] > x.shape[-1] else y
+
+
+def _far(got, want):
+    got, want = got.cpu().double(), want.double()
+    return ((got - want).norm() / want.norm()).item()
+
+
+def _allowed(x, dtype, gram):
+    """How far a kernel's result may be from the one in 64 bits, by norms."""
+    half = torch.finfo(dtype).eps / 2
+    if gram:
+        # Everything in 64 bits until the result's rounding. An inner product
+        # of K terms is off by K 2^-53 at most, and a change of G_0 comes out
+        # at most a^(3 steps - 3) |b| a^2 1.1 = 1.5e7 times as large.
+        return half + max(x.shape[-2:]) * 2.0 ** -53 * 1.5e7 * 2
+    if dtype == torch.bfloat16:
+        # the result's rounding, and as much again for the Gram matrices in
+        # 11 bits: 5 steps, each of 2^-12 times |b| < 5 at most
+        return half + 25 * 2.0 ** -12
+    # hi + lo hold a value within 2^-23, and a product leaves out lo lo below
+    # 2^-22 of the values: together at most 4 times what float32 (2^-24) does
+    # to each; `_iterate` in float32 shows how the steps raise that
+    return half + 4 * _far(_iterate(x.float(), torch.float32),
+                           _iterate(x, torch.float64)) + 20 * 2.0 ** -24
+
+
+def _check(x, steps=5, c=COEFFICIENTS):
+    want = _iterate(x, torch.float64, steps, c)
+    got = ops.newton_schulz(x.cuda(), steps, c)
+    assert got.shape == x.shape and got.dtype == x.dtype
+    assert got.is_contiguous() and got.device.type == "cuda"
+    gram = min(x.shape[-2:]) <= 128
+    far = _far(got, want)
+    assert far <= _allowed(x, x.dtype, gram), far
+
+
+# ------------------------------------------------------------------ CPU
+
+@pytest.mark.parametrize("shape", [(1, 1), (5, 5), (4, 9), (30, 7), (2, 6, 9),
+                                   (3, 8, 2)])
+def test_definition(shape):
+    x = _matrix(*shape)
+    got = ops.newton_schulz(x)
+    # the 64-bit forms agree to far below the result's rounding
+    assert _far(got, _by_singular_values(x)) < 2.0 ** -23
+    assert got.shape == x.shape and got.is_contiguous()
+
+
+def test_small_singular_values_come_near_one():
+    s = torch.linalg.svdvals(ops.newton_schulz(_matrix(40, 100)).double())
+    assert 0.6 < s.min() and s.max() < 1.25
+    x = _matrix(20, 50)
+    y = ops.newton_schulz(x, 25, (1.875, -1.25, 0.375)).double()
+    assert (y @ y.t() - torch.eye(20)).abs().max() < 1e-5
+
+
+def test_scale_and_transpose_do_not_matter():
+    x = _matrix(12, 31)
+    y = ops.newton_schulz(x)
+    assert torch.equal(ops.newton_schulz(x * 2.0 ** 90), y)
+    assert torch.equal(ops.newton_schulz(x.t()), y.t())
+
+
+def _special(device):
+    x = _matrix(3, 6, 9)
+    x[0] = 0
+    x[2, 4, 4] = float("inf")
+    y = ops.newton_schulz(x.to(device)).cpu()
+    assert not y[0].any() and y[1].isfinite().all() and y[1].any()
+    assert y[2].isnan().all()
+    for shape in [(0, 5), (5, 0), (0, 4, 4), (3, 0, 2)]:
+        assert ops.newton_schulz(torch.ones(shape, device=device)
+                                 ).shape == shape
+
+
+def test_special_values():
+    _special("cpu")
+
+
+def test_refusals():
+    x = torch.ones(3, 4)
+    for bad in (0, -1, 1.5, 2000, True):
+        with pytest.raises(ValueError, match="steps"):
+            ops.newton_schulz(x, bad)
+    for bad in ((1.0, 2.0), (1.0, 2.0, float("nan")), (1, 2, 3, 4)):
+        with pytest.raises(ValueError, match="coefficients"):
+            ops.newton_schulz(x, 5, bad)
+    with pytest.raises(ValueError, match="3-D"):
+        ops.newton_schulz(torch.ones(3))
+    with pytest.raises(TypeError, match="float32"):
+        ops.newton_schulz(x.double())
+    A = from_numpy(np.ones((300, 129), dtype=np.float32))
+    with pytest.raises(ValueError, match="128"):
+        newton_schulz_panel(A)
+    with pytest.raises(ValueError, match="128"):
+        svd_compressed(A, 125, normalizer="newton_schulz")
+    with pytest.raises(ValueError, match="normalizer"):
+        svd_compressed(A, 5, normalizer="LU")
+
+
+def _panel(m=400, k=12, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(m, k, generator=g) * torch.logspace(0, -2, k)
+
+
+def test_panel_is_the_same_iteration():
+    x = _panel()
+    got = newton_schulz_panel(from_numpy(x.numpy())).local
+    assert _far(got, _iterate(x, torch.float64)) < 2.0 ** -23
+
+
+def _panel_on_ranks(rank, world):
+    from mi355ml.parallel import comm
+    x = _panel(101)
+    lo, hi = (0, 3) if rank == 0 else (3, 101)   # fewer rows than columns
+    got = newton_schulz_panel(DistArray(x[lo:hi].contiguous(), 101, lo,
+                                        comm.default()))
+    want = _iterate(x, torch.float64)[lo:hi]
+    assert got.global_rows == 101 and got.row_offset == lo
+    assert (got.local.double() - want).abs().max() < 1e-6
+
+
+def test_panel_spread_over_ranks(mp_runner):
+    mp_runner(_panel_on_ranks, world=2)
+
+
+def _decaying(m=600, d=80, seed=2):
+    rng = np.random.default_rng(seed)
+    u, _ = np.linalg.qr(rng.standard_normal((m, d)))
+    v, _ = np.linalg.qr(rng.standard_normal((d, d)))
+    s = 0.8 ** np.arange(d)
+    return ((u * s) @ v.T * 10).astype(np.float32), s * 10
+
+
+def _check_range_finder(device):
+    x, s = _decaying()
+    X = from_numpy(x)
+    assert device is None or X.device.type == device
+    _, got, vh = svd_compressed(X, 10, n_power_iter=3, compute_u=False,
+                                normalizer="newton_schulz")
+    _, qr, vq = svd_compressed(X, 10, n_power_iter=3, compute_u=False)
+    # A power iteration of q steps leaves (s_21 / s_i)^(2q+1) of the
+    # neglected directions in the i-th one and its square in the value: below
+    # 1e-6 for i <= 6 here. What is left is float32's rounding of the products
+    # (about 1e-6 of s_1, and s_6 = s_1 / 3).
+    np.testing.assert_allclose(got[:6].cpu(), s[:6], rtol=2e-5)
+    np.testing.assert_allclose(got.cpu(), qr.cpu(), rtol=1e-3)
+    same = (vh[:4] * vq[:4]).sum(dim=1).abs().cpu()
+    assert (same > 1 - 1e-4).all()
+
+
+def test_range_finder():
+    _check_range_finder(None)
+
+
+def test_estimators_take_the_normalizer():
+    x, s = _decaying()
+    X = from_numpy(x)
+    t = TruncatedSVD(5, algorithm="randomized",
+                     power_iteration_normalizer="newton_schulz").fit(X)
+    np.testing.assert_allclose(t.singular_values_, s[:5], rtol=1e-4)
+    p = PCA(5, svd_solver="randomized", iterated_power=4,
+            power_iteration_normalizer="newton_schulz").fit(X)
+    q = PCA(5, svd_solver="full").fit(X)
+    np.testing.assert_allclose(p.singular_values_, q.singular_values_,
+                               rtol=1e-4)
+    with pytest.raises(ValueError, match="normalizer"):
+        TruncatedSVD(5, algorithm="randomized",
+                     power_iteration_normalizer="LU").fit(X)
+
+
+# ------------------------------------------------------------------ GPU
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 50), (50, 1), (16, 16),
+                                   (17, 15), (33, 130), (130, 48), (60, 3001),
+                                   (2999, 77), (96, 97), (112, 300),
+                                   (500, 113), (128, 128), (127, 5000)])
+def test_gpu_gram_way(shape, dtype):
+    _check(_matrix(*shape, dtype=dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shape", [(129, 129), (130, 700), (701, 129),
+                                   (192, 192), (257, 300), (300, 1000),
+                                   (1023, 400), (640, 640)])
+def test_gpu_products(shape, dtype):
+    _check(_matrix(*shape, dtype=dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(3, 20, 50), (5, 64, 40), (300, 4, 4),
+                                   (3, 200, 150), (2, 140, 333),
+                                   (17, 130, 260), (2, 1500, 1100)])
+def test_gpu_batches(shape, dtype):
+    x = _matrix(*shape, dtype=dtype)
+    x[1] *= 1e3   # each matrix has a norm of its own
+    _check(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(40, 90), (200, 260)])
+@pytest.mark.parametrize("steps,c", [(1, COEFFICIENTS), (2, COEFFICIENTS),
+                                     (3, (1.5, -0.5, 0.0)),
+                                     (4, (2.0, -1.5, 0.5)),
+                                     (2, (3.0, 0.0, 0.0)),
+                                     (8, (1.875, -1.25, 0.375))])
+def test_gpu_steps_and_coefficients(shape, steps, c):
+    x = _matrix(*shape)
+    want = _iterate(x, torch.float64, steps, c)
+    far = _far(ops.newton_schulz(x.cuda(), steps, c), want)
+    f32 = _far(_iterate(x, torch.float32, steps, c), want)
+    assert far <= 2.0 ** -24 + 4 * f32 + 4 * steps * 2.0 ** -24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [30, 150])
+def test_gpu_ranges(n):
+    # any scale that float32 holds, subnormal numbers among it
+    x = _matrix(n, n + 20, scale=1.0)
+    want = ops.newton_schulz(x.cuda())
+    for e in (-60, 60, 120):
+        assert torch.equal(ops.newton_schulz(x.cuda() * 2.0 ** e), want)
+    _check(x * 1e-38)
+
+
+@pytest.mark.gpu
+def test_gpu_special_values():
+    _special("cuda")
+    x = _matrix(3, 150, 200)
+    x[0] = 0
+    x[2, 4, 4] = float("nan")
+    y = ops.newton_schulz(x.cuda()).cpu()
+    assert not y[0].any() and y[1].isfinite().all() and y[1].any()
+    assert y[2].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [40, 140])
+def test_gpu_strides(n):
+    big = _matrix(2, n + 9, 2 * n + 30).cuda()
+    views = [big[:, 3:n, 5:], big[0].t(), big[1, :, ::2], big[:, ::2, 1:n],
+             big.transpose(0, 1)[:, :, :n], big[:1].expand(3, -1, -1),
+             big[0, :1].expand(n, -1)]
+    for v in views:
+        want = ops.newton_schulz(v.contiguous())
+        assert torch.equal(ops.newton_schulz(v), want)
+
+
+@pytest.mark.gpu
+def test_gpu_same_bits_every_time():
+    for shape in [(100000, 60), (700, 600)]:
+        x = _matrix(*shape).cuda()
+        first = ops.newton_schulz(x)
+        for _ in range(3):
+            assert torch.equal(ops.newton_schulz(x), first)
+
+
+@pytest.mark.gpu
+def test_gpu_panel_is_newton_schulz():
+    x = _panel(5000, 60)
+    A = from_numpy(x.numpy())
+    got = newton_schulz_panel(A).local
+    assert torch.equal(got, ops.newton_schulz(x.cuda()))
+    few = _panel(20, 50)                  # fewer rows than columns
+    got = newton_schulz_panel(from_numpy(few.numpy())).local
+    assert _far(got, _iterate(few, torch.float64)) < 1e-6
+
+
+@pytest.mark.gpu
+def test_gpu_range_finder():
+    _check_range_finder("cuda")
+
+
+@pytest.mark.gpu
+def test_gpu_divergence_is_refused():
+    x = _matrix(200, 200).cuda()
+    with pytest.raises(RuntimeError, match="diverge"):
+        ops.newton_schulz(x, 50, (50.0, 50.0, 50.0))
+
+
+@pytest.mark.gpu
+def test_gpu_other_stream_and_graph():
+    shapes = [(2000, 50), (300, 200)]
+    xs = [_matrix(*s).cuda() for s in shapes]
+    want = [ops.newton_schulz(x) for x in xs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [ops.newton_schulz(x) for x in xs]
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    static, graphs = [x.clone() for x in xs], []
+    for x in static:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.newton_schulz(x)
+        graphs.append((graph, out))
+    for seed in range(4):
+        new = [_matrix(*s, seed=seed + 5).cuda() for s in shapes]
+        for a, b in zip(static, new):
+            a.copy_(b)
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, out), x in zip(graphs, new):
+            assert torch.equal(out, ops.newton_schulz(x))
