@@ -267,10 +267,11 @@ __device__ __forceinline__ void store4(const Scales& e, long m, long n,
 }
 
 // `slab` not null: the sums of this split of K, for joining later.
-template <class T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void int8_tile_k(
+template <class T, int BM, int WM, int WN, int STAGES>
+__global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void int8_tile_k(
     Sources s, Scales e, int tm, int tn, int per, int* __restrict__ slab) {
-  typedef Tile<v4i, BM, BN, WM, WN> P;
+  constexpr int BN = BM;
+  typedef Tile<v4i, BM, BN, WM, WN, STAGES> P;
   __shared__ __attribute__((aligned(16))) char lds[P::kLds];
   int ti, tj;
   banded(xcd_contiguous(blockIdx.x, gridDim.x), tm, tn, ti, tj);
@@ -391,8 +392,7 @@ Plan plan_of(long m, long n, long k) {
     p.tm = 1;
     p.tn = (int)((n + 15) / 16);
   } else {
-    const long big = ((m + 127) / 128) * ((n + 127) / 128);
-    p.kind = big >= 256 ? 128 : 64;
+    p.kind = tile_size(m, n, 1, false);
     p.tm = (int)((m + p.kind - 1) / p.kind);
     p.tn = (int)((n + p.kind - 1) / p.kind);
   }
@@ -413,16 +413,17 @@ void product(const Sources& s, const Scales& e, const Plan& p, int* slab,
 #define FEW(MT)                                                            \
   hipLaunchKernelGGL((int8_few_rows_k<T, MT>), grid, dim3(256), 0, st, s, \
                      e, p.per, slab)
-#define TILE(BM, BN, WM, WN)                                              \
-  hipLaunchKernelGGL((int8_tile_k<T, BM, BN, WM, WN>), grid,              \
-                     dim3((BM / WM) * (BN / WN) * 64), 0, st, s, e, p.tm, \
+#define TILE(BM, WM, WN, STAGES)                                          \
+  hipLaunchKernelGGL((int8_tile_k<T, BM, WM, WN, STAGES>), grid,          \
+                     dim3((BM / WM) * (BM / WN) * 64), 0, st, s, e, p.tm, \
                      p.tn, p.per, slab)
   switch (p.kind) {
     case 1: FEW(1); break;
     case 2: FEW(2); break;
     case 4: FEW(4); break;
-    case 64: TILE(64, 64, 32, 32); break;
-    default: TILE(128, 128, 64, 64);
+    case 64: TILE(64, 32, 32, 2); break;
+    case 128: TILE(128, 64, 32, 2); break;
+    default: TILE(256, 128, 64, 2);
   }
 #undef FEW
 #undef TILE

@@ -467,10 +467,10 @@ __global__ __launch_bounds__(256) void split_k(
 // result.
 enum { kHalves, kFloat, kFp16, kBf16 };
 
-template <int OUT, int BM, int WM>
-__global__ __launch_bounds__((BM / WM) * (BM / WM) * 64) void step_k(
+template <int OUT, int BM, int WM, int WN, int STAGES>
+__global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void step_k(
     Sources s, Step p) {
-  typedef Tile<v4f, BM, BM, WM, WM> P;
+  typedef Tile<v4f, BM, BM, WM, WN, STAGES> P;
   __shared__ __attribute__((aligned(16))) char lds[P::kLds];
   int ti, tj;
   const int b = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -482,8 +482,8 @@ __global__ __launch_bounds__((BM / WM) * (BM / WM) * 64) void step_k(
          s.parts * ((s.kbytes + kStep - 1) / kStep), lds, acc);
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
-  const int wm0 = ti * BM + wave / (BM / WM) * WM;
-  const int wn0 = tj * BM + wave % (BM / WM) * WM;
+  const int wm0 = ti * BM + wave / (BM / WN) * WM;
+  const int wn0 = tj * BM + wave % (BM / WN) * WN;
   const int c = lane & 15, h = lane >> 4;
   const int rows = s.rows_a, cols = s.rows_b;
   float alpha = p.alpha, beta = p.beta;
@@ -574,17 +574,26 @@ __global__ __launch_bounds__((BM / WM) * (BM / WM) * 64) void step_k(
 
 template <int OUT>
 void step_as(Sources s, Step p, int batch, hipStream_t st) {
-  // 128 x 128 tiles once they fill the chip, 64 x 64 ones below
-  const long m128 = (s.rows_a + 127) / 128, n128 = (s.rows_b + 127) / 128;
-  const long count = (p.symmetric ? m128 * (m128 + 1) / 2 : m128 * n128);
-  const int size = count * batch >= 256 ? 128 : 64;
+  const int size = tile_size(s.rows_a, s.rows_b, batch, p.symmetric);
   p.tm = (s.rows_a + size - 1) / size;
   p.tn = (s.rows_b + size - 1) / size;
-  const dim3 grid(p.symmetric ? p.tm * (p.tm + 1) / 2 : p.tm * p.tn, batch);
-  if (size == 128)
-    hipLaunchKernelGGL((step_k<OUT, 128, 64>), grid, dim3(256), 0, st, s, p);
+  const int tiles = p.symmetric ? p.tm * (p.tm + 1) / 2 : p.tm * p.tn;
+  const dim3 grid(tiles, batch);
+#define STEP(BM, WM, WN, STAGES)                                 \
+  hipLaunchKernelGGL((step_k<OUT, BM, WM, WN, STAGES>), grid,    \
+                     dim3((BM / WM) * (BM / WN) * 64), 0, st, s, p)
+  if (size == 256)
+    STEP(256, 128, 64, 2);
+  else if (size == 128 && (long)tiles * batch <= 256)
+    // a CU's only workgroup: four steps in LDS (2048^2 outputs of K = 6144:
+    // 56 us, with two steps 70), otherwise two so that two workgroups fit
+    // (4096^2 of K = 4096: 150 us, with four steps 170)
+    STEP(128, 64, 32, 4);
+  else if (size == 128)
+    STEP(128, 64, 32, 2);
   else
-    hipLaunchKernelGGL((step_k<OUT, 64, 32>), grid, dim3(256), 0, st, s, p);
+    STEP(64, 32, 32, 2);
+#undef STEP
 }
 
 template <class T, int NT>

@@ -4,7 +4,7 @@
 // a row each, from the same places, so that one loader, one LDS layout and
 // one loop serve both types.
 //
-// A workgroup computes a BM x BN tile in steps of 128 bytes of K. The step's
+// A workgroup computes a BM x BN tile in steps of 128 bytes of K. A step's
 // rows go to LDS by DMA (global_load_lds, 16 bytes a lane), which writes
 // lanes in order; the XOR swizzle that keeps ds_read_b128 free of bank
 // conflicts (chunk c of row r sits in place c ^ (r & 7)) is therefore put
@@ -78,16 +78,48 @@ __device__ __forceinline__ v4f mma(v4i x, v4i y, v4f c) {
       __builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0, 0);
 }
 
+template <int N> struct Count { static constexpr int value = N; };
+
 // BM x BN: the workgroup's tile, WM x WN: a wave's. ACC is v4i for 8-bit
-// integers and v4f for 16-bit floats.
-template <class ACC, int BM, int BN, int WM, int WN>
+// integers and v4f for 16-bit floats. STAGES steps fit in LDS, all but one of
+// them on their way.
+//
+// Measured (us for one step of one tile on each of the 256 CUs, from products
+// of 4096^2 and 2048^2 outputs): 256 x 256 by 8 waves 1.75, 128 x 128 by 8
+// waves 0.58, 64 x 64 by 4 waves 0.22 (0.36 where a CU has no second
+// workgroup). So for the same output 256 x 256 tiles take 3/4 of the time of
+// 128 x 128 ones and half of that of 64 x 64 ones, as long as they fill the
+// chip; tile_size weighs that. At 4096^3 a product of fp16 runs at 1.2
+// PFLOP/s and one of int8 at 2.6 POP/s (the library: 1.1 and 2.05). At that
+// point the matrix cores are busy 60% of the time at a clock that the power
+// limit holds at 1.75 GHz; LDS is at a quarter of its rate.
+template <class ACC, int BM, int BN, int WM, int WN, int STAGES>
 struct Tile {
   static constexpr int kWaves = (BM / WM) * (BN / WN);
   static constexpr int kThreads = kWaves * 64;
   static constexpr int MI = WM / 16, NJ = WN / 16;
   static constexpr int kStage = (BM + BN) * kStep;
-  static constexpr int kLds = 2 * kStage;
+  static constexpr int kLds = STAGES * kStage;
   static constexpr bool kInt = __is_same(ACC, v4i);
+
+  // Spreads a half's reads from LDS, and V loads from memory, over the
+  // multiplications, one at a time: left to itself the compiler puts the
+  // reads behind the multiplications and then waits for them.
+  template <int V>
+  static __device__ __forceinline__ void interleave() {
+    constexpr int R = MI + NJ, M = MI * NJ, EACH = M / (R + V);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, M - EACH * (R + V), 0);
+  }
 
   // acc[i][j][r] is the sum for row  m = i * 16 + lane % 16  and column
   // n = j * 16 + lane / 16 * 4 + r  of the wave's part of the tile: B goes in
@@ -118,13 +150,18 @@ struct Tile {
     const long at_a = batch * s.batch_a + (long)m0 * s.row_a;
     const long at_b = batch * s.batch_b + (long)n0 * s.row_b;
 
-    auto load = [&](int t, int buf) {
-      const int part = t / steps, k = t - part * steps;
-      const char* pa = s.a[part] + at_a + (long)k * kStep;
-      const char* pb = s.b[part] + at_b + (long)k * kStep;
+    // where the next step is loaded from
+    const char* pa = s.a[0] + at_a + (long)(first % steps) * kStep;
+    const char* pb = s.b[0] + at_b + (long)(first % steps) * kStep;
+    int k = first % steps, part = 0;
+    // from the end of one part to the beginning of the next
+    const long back = (long)steps * kStep - kStep;
+    const long a1 = s.a[1] - s.a[0] - back, a2 = s.a[2] - s.a[1] - back;
+    const long b1 = s.b[1] - s.b[0] - back, b2 = s.b[2] - s.b[1] - back;
+    auto load = [&](int buf) {
       // a chunk that begins behind the row's end is read from the step's
       // first one instead, and masked below
-      const unsigned c = (k == steps - 1 && c16 >= tail) ? 0 : c16;
+      const unsigned c = kInt && k == steps - 1 && c16 >= tail ? 0 : c16;
       char* la = lds + buf * kStage + wave * 1024;
       char* lb = la + BM * kStep;
 #pragma unroll
@@ -139,48 +176,117 @@ struct Tile {
             (const __attribute__((address_space(1))) void*)(pb + (ob[i] + c)),
             (__attribute__((address_space(3))) void*)(lb + i * kWaves * 1024),
             16, 0, 0);
+      const bool wrap = ++k == steps;
+      k = wrap ? 0 : k;
+      pa += wrap ? (part ? a2 : a1) : (long)kStep;
+      pb += wrap ? (part ? b2 : b1) : (long)kStep;
+      part += wrap;
     };
-
+    const char* base_a = lds + (wm * WM + (lane & 15)) * kStep;
+    const char* base_b = lds + (BM + wn * WN + (lane & 15)) * kStep;
+    // 64 bytes of each row: one operand of each matrix instruction
+    struct Half { v4i a[MI], b[NJ]; };
+    auto fetch = [&](Half& f, int buf, int kk) {
+      const int at = buf * kStage +
+                     ((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 16;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+        f.a[i] = *(const v4i*)(base_a + at + i * 16 * kStep);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        f.b[j] = *(const v4i*)(base_b + at + j * 16 * kStep);
+    };
+    auto multiply = [&](const Half& f) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          acc[i][j] = mma(f.b[j], f.a[i], acc[i][j]);
+    };
+    // All loads but the last N steps' are in, and every wave is done with
+    // the buffer of the step before.
+    auto turn = [&](auto n) {
+      constexpr int LEFT = decltype(n)::value * (LA + LB);
+      // vmcnt in bits 0-3 and 14-15, lgkmcnt 0, expcnt not waited for
+      constexpr int IMM = (LEFT & 15) | ((LEFT >> 4) << 14) | (7 << 4);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(IMM);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[i][j] = ACC{0, 0, 0, 0};
 
-    const int row = (lane & 15) * kStep;
-    load(first, 0);
-    for (int t = first; t < last; ++t) {
-      const int buf = (t - first) & 1;
-      // one barrier a step: the loads of this step are in, and every wave
-      // has read the other buffer
-      __syncthreads();
-      if (t + 1 < last) load(t + 1, buf ^ 1);
-      const char* la = lds + buf * kStage + wm * WM * kStep + row;
-      const char* lb = lds + buf * kStage + (BM + wn * WN) * kStep + row;
-      const bool cut = kInt && tail < kStep && t % steps == steps - 1;
+    // A step's two halves of 64 bytes are multiplied while the next half is
+    // on its way from LDS, across the turn of the buffers too: the matrix
+    // cores wait for nothing but the barrier. A buffer is loaded again right
+    // after the turn that frees it, a whole step before it is read.
+    // A step's two halves are multiplied while the next half is on its way
+    // from LDS, across the turn of the buffers too, so that the matrix cores
+    // wait for nothing but the barrier (one a step). A buffer is loaded again
+    // right after the turn that frees it.
+    Half f0, f1;
+    const int count = last - first;
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const int chunk = kk * 4 + (lane >> 4);
-        const int place = (chunk ^ (lane & 7)) * 16;
-        v4i fa[MI], fb[NJ];
+    for (int u = 0; u < STAGES; ++u)
+      if (u < count) load(u);
+    if (count >= STAGES) turn(Count<STAGES - 1>());
+    else turn(Count<0>());
+    fetch(f0, 0, 0);
+    int buf = 0;
+    auto after = [](int b) { return b + 1 == STAGES ? 0 : b + 1; };
+    int t = 0;
+    for (; t + STAGES < count; ++t) {
+      fetch(f1, buf, 1);
+      multiply(f0);
+      interleave<0>();
+      turn(Count<STAGES - 2>());
+      const int next = after(buf);
+      fetch(f0, next, 0);
+      load(buf);
+      multiply(f1);
+      interleave<LA + LB>();
+      buf = next;
+    }
+    for (; t + 1 < count; ++t) {
+      fetch(f1, buf, 1);
+      multiply(f0);
+      interleave<0>();
+      turn(Count<0>());
+      buf = after(buf);
+      fetch(f0, buf, 0);
+      multiply(f1);
+      interleave<0>();
+    }
+    fetch(f1, buf, 1);
+    if (kInt && tail < kStep && last % steps == 0) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
-          fa[i] = *(const v4i*)(la + i * 16 * kStep + place);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-          fb[j] = *(const v4i*)(lb + j * 16 * kStep + place);
-        if (cut)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j)
-            fb[j] = keep_bytes(fb[j], tail - chunk * 16);
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j)
-            acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
+      for (int j = 0; j < NJ; ++j) {
+        f0.b[j] = keep_bytes(f0.b[j], tail - (lane >> 4) * 16);
+        f1.b[j] = keep_bytes(f1.b[j], tail - 64 - (lane >> 4) * 16);
       }
     }
+    multiply(f0);
+    multiply(f1);
     __syncthreads();
   }
 };
+
+// The tile that needs the least time for the outputs of one launch: time for
+// a round of one tile on each CU, times the rounds.
+inline int tile_size(long m, long n, long batch, bool symmetric) {
+  auto rounds = [&](long size) {
+    const long tm = (m + size - 1) / size, tn = (n + size - 1) / size;
+    const long tiles = batch * (symmetric ? tm * (tm + 1) / 2 : tm * tn);
+    return (double)((tiles + 255) / 256);
+  };
+  const double t256 = 1.75 * rounds(256), t128 = 0.58 * rounds(128);
+  const double t64 = rounds(64) > 1 ? 0.22 * rounds(64) : 0.36;
+  return t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+}
 
 }  // namespace tile_product
