@@ -20,7 +20,8 @@ void launch_factor(const double*, int, int, double, double, double, int,
 void launch_apply(const void*, int, int, long, int, long, long, int,
                   const double*, void*, long, long, hipStream_t);
 void launch_split(const void*, int, int, int, long, long, int, double*, int,
-                  Halves, Halves, float*, hipStream_t);
+                  Halves, Halves, Halves, Halves, Halves, float*,
+                  hipStream_t);
 void launch_step(Halves, int, Halves, int, int, int, Step, int, int,
                  hipStream_t);
 }
@@ -186,7 +187,7 @@ torch::Tensor by_products(const Matrices& v, int steps, double a, double b,
   const auto st = stream_of(v.x);
   launch_split(v.x.data_ptr(), v.type, (int)v.rows, (int)v.cols, v.ld,
                v.stride, (int)batch, squares.data_ptr<double>(), parts, x, xt,
-               factor.data_ptr<float>(), st);
+               xt_next, g, poly, factor.data_ptr<float>(), st);
 
   double bound = 1.0;  // of the singular values of X
   int ex = 14;         // stored values are 2^ex times the true ones

@@ -11,6 +11,8 @@
 #include <hip/hip_fp16.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "tile_product.h"
 
 using namespace tile_product;
@@ -380,28 +382,43 @@ __global__ __launch_bounds__(256) void int8_join_k(
                                   e.bias ? e.bias[n] : 0.0f));
 }
 
-struct Plan { int kind, tm, tn, splits, per; };
+// How a product is computed: by `rows` (16, 32 or 64) rows without LDS, or in
+// square tiles of `size`, each with K in `splits` parts of `per` steps.
+struct Plan { int rows, size, tm, tn, splits, per; };
 
-// Which kernel, and over how many parts of K. Parts are made until the chip
-// has two workgroups for each CU, but none shorter than 4 steps.
 Plan plan_of(long m, long n, long k) {
-  Plan p;
+  Plan p = {};
   const int steps = (int)((k + kStep - 1) / kStep);
   if (m <= 64) {
-    p.kind = m <= 16 ? 1 : m <= 32 ? 2 : 4;
+    // enough workgroups for two on each CU, of 16 steps at least
+    p.rows = m <= 16 ? 16 : m <= 32 ? 32 : 64;
     p.tm = 1;
     p.tn = (int)((n + 15) / 16);
+    long want = p.tn >= 512 ? 1 : (512 + p.tn - 1) / p.tn;
+    want = std::min(want, std::min(64L, std::max(1L, (long)steps / 16)));
+    p.per = (int)((steps + want - 1) / want);
   } else {
-    p.kind = tile_size(m, n, 1, false);
-    p.tm = (int)((m + p.kind - 1) / p.kind);
-    p.tn = (int)((n + p.kind - 1) / p.kind);
+    // the tile and the split that need the least time; joining the parts
+    // takes a launch, and writes and reads them at 4 TB/s
+    double best = 1e30;
+    for (const TileCost& c : kTiles)
+      for (int splits = 1; splits <= 64 && splits * 4 <= steps + 3;
+           splits *= 2) {
+        const long tm = (m + c.size - 1) / c.size;
+        const long tn = (n + c.size - 1) / c.size;
+        const int per = (steps + splits - 1) / splits;
+        const double join =
+            splits > 1 ? 4.0 + 8e-6 * splits * m * n / 4.0 : 0.0;
+        const double t = per * step_time(c, tm * tn * splits) + join;
+        if (t < best) {
+          best = t;
+          p.size = c.size;
+          p.tm = (int)tm;
+          p.tn = (int)tn;
+          p.per = per;
+        }
+      }
   }
-  const long tiles = (long)p.tm * p.tn;
-  long want = tiles >= 512 ? 1 : (512 + tiles - 1) / tiles;
-  const long most = steps / 16 > 1 ? steps / 16 : 1;
-  if (want > most) want = most;
-  if (want > 64) want = 64;
-  p.per = (int)((steps + want - 1) / want);
   p.splits = (steps + p.per - 1) / p.per;
   return p;
 }
@@ -410,20 +427,19 @@ template <class T>
 void product(const Sources& s, const Scales& e, const Plan& p, int* slab,
              hipStream_t st) {
   const dim3 grid(p.tm * p.tn, p.splits);
-#define FEW(MT)                                                            \
+#define FEW(MT)                                                           \
   hipLaunchKernelGGL((int8_few_rows_k<T, MT>), grid, dim3(256), 0, st, s, \
                      e, p.per, slab)
 #define TILE(BM, WM, WN, STAGES)                                          \
   hipLaunchKernelGGL((int8_tile_k<T, BM, WM, WN, STAGES>), grid,          \
                      dim3((BM / WM) * (BM / WN) * 64), 0, st, s, e, p.tm, \
                      p.tn, p.per, slab)
-  switch (p.kind) {
-    case 1: FEW(1); break;
-    case 2: FEW(2); break;
-    case 4: FEW(4); break;
-    case 64: TILE(64, 32, 32, 2); break;
-    case 128: TILE(128, 64, 32, 2); break;
-    default: TILE(256, 128, 64, 2);
+  if (p.rows == 16) FEW(1);
+  else if (p.rows == 32) FEW(2);
+  else if (p.rows == 64) FEW(4);
+  else {
+    const bool alone = (long)p.tm * p.tn * p.splits <= 256;
+    BY_TILE_SIZE(p.size, alone, TILE)
   }
 #undef FEW
 #undef TILE

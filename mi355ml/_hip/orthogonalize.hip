@@ -409,7 +409,7 @@ template <class T>
 __global__ __launch_bounds__(256) void split_k(
     const T* __restrict__ x, int rows, int cols, long ld, long batch_x,
     int tall, const double* __restrict__ part, int parts, Halves d, Halves t,
-    float* __restrict__ factor) {
+    Halves t2, Halves g, Halves poly, float* __restrict__ factor) {
   __shared__ float tile[64][65];
   __shared__ double sum[4];
   const int lane = threadIdx.x & 63;
@@ -427,6 +427,21 @@ __global__ __launch_bounds__(256) void split_k(
   if (blockIdx.x == 0 && threadIdx.x == 0)
     factor[blockIdx.y] =
         !fine ? NAN : norm > 0.0 ? (float)(1.0 / frac) : 0.0f;
+  // what the products read behind the last column has to be zeros
+  auto clear = [&](const Halves& o, int rows, int cols) {
+    const int width = (int)o.ld - cols;
+    for (long i = blockIdx.x * 256 + threadIdx.x; i < (long)rows * width;
+         i += gridDim.x * 256) {
+      const long at = blockIdx.y * o.batch + i / width * o.ld + cols +
+                      i % width;
+      o.hi[at] = 0;
+      if (o.lo) o.lo[at] = 0;
+    }
+  };
+  const int n = tall ? cols : rows, m = tall ? rows : cols;
+  clear(t2, m, n);
+  clear(g, n, n);
+  clear(poly, n, n);
   x += blockIdx.y * batch_x;
   // the tile in the input's own layout
   const int across_tiles = (cols + 63) / 64;
@@ -525,7 +540,7 @@ __global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void step_k(
           hi[r] = (_Float16)v[r];
           lo[r] = (_Float16)(v[r] - (float)hi[r]);
         }
-        if (p.d.hi && m < rows && n < p.d.ld) {
+        if (p.d.hi && m < rows && n < cols) {
           const long at = z * p.d.batch + (long)m * p.d.ld + n;
           *(v4h*)(p.d.hi + at) = hi;
           if (p.d.lo) *(v4h*)(p.d.lo + at) = lo;
@@ -556,11 +571,12 @@ __global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void step_k(
       // keep them so
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-      for (int u = 0; u < 16 * (WM / 8) / 64; ++u) {
+      for (int u = 0; u < (16 * (WM / 8) + 63) / 64; ++u) {
         const int k = u * 64 + lane;
+        if (k >= 16 * (WM / 8)) continue;
         const int row = k / (WM / 8), m = wm0 + k % (WM / 8) * 8;
         const int nn = wn0 + j * 16 + row;
-        if (nn < cols && m < p.t.ld) {
+        if (nn < cols && m < rows) {
           const long at = z * p.t.batch + (long)nn * p.t.ld + m;
           *(v8h*)(p.t.hi + at) = *(const v8h*)(th + row * LD + m - wm0);
           if (p.t.lo)
@@ -574,25 +590,28 @@ __global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void step_k(
 
 template <int OUT>
 void step_as(Sources s, Step p, int batch, hipStream_t st) {
-  const int size = tile_size(s.rows_a, s.rows_b, batch, p.symmetric);
+  auto tiles_of = [&](int size) {
+    const long tm = (s.rows_a + size - 1) / size;
+    const long tn = (s.rows_b + size - 1) / size;
+    return p.symmetric ? tm * (tm + 1) / 2 : tm * tn;
+  };
+  int size = 0;
+  double best = 0;
+  for (const TileCost& c : kTiles) {
+    const double t = step_time(c, tiles_of(c.size) * batch);
+    if (!size || t < best) {
+      size = c.size;
+      best = t;
+    }
+  }
   p.tm = (s.rows_a + size - 1) / size;
   p.tn = (s.rows_b + size - 1) / size;
-  const int tiles = p.symmetric ? p.tm * (p.tm + 1) / 2 : p.tm * p.tn;
-  const dim3 grid(tiles, batch);
+  const bool alone = tiles_of(size) * batch <= 256;
+  const dim3 grid((unsigned)tiles_of(size), batch);
 #define STEP(BM, WM, WN, STAGES)                                 \
   hipLaunchKernelGGL((step_k<OUT, BM, WM, WN, STAGES>), grid,    \
                      dim3((BM / WM) * (BM / WN) * 64), 0, st, s, p)
-  if (size == 256)
-    STEP(256, 128, 64, 2);
-  else if (size == 128 && (long)tiles * batch <= 256)
-    // a CU's only workgroup: four steps in LDS (2048^2 outputs of K = 6144:
-    // 56 us, with two steps 70), otherwise two so that two workgroups fit
-    // (4096^2 of K = 4096: 150 us, with four steps 170)
-    STEP(128, 64, 32, 4);
-  else if (size == 128)
-    STEP(128, 64, 32, 2);
-  else
-    STEP(64, 32, 32, 2);
+  BY_TILE_SIZE(size, alone, STEP)
 #undef STEP
 }
 
@@ -710,7 +729,8 @@ extern "C" void launch_apply(const void* x, int dtype, int wide, long length,
 
 extern "C" void launch_split(const void* x, int dtype, int rows, int cols,
                              long ld, long batch_x, int batch, double* part,
-                             int parts, Halves d, Halves t, float* factor,
+                             int parts, Halves d, Halves t, Halves t2,
+                             Halves g, Halves poly, float* factor,
                              hipStream_t st) {
   const int tall = rows > cols;
   const dim3 grid(((cols + 63) / 64) * ((rows + 63) / 64), batch);
@@ -718,8 +738,8 @@ extern "C" void launch_split(const void* x, int dtype, int rows, int cols,
   hipLaunchKernelGGL((squares_k<T>), dim3(parts, batch), dim3(256), 0, st,  \
                      (const T*)x, rows, cols, ld, batch_x, part);           \
   hipLaunchKernelGGL((split_k<T>), grid, dim3(256), 0, st, (const T*)x,     \
-                     rows, cols, ld, batch_x, tall, part, parts, d, t,      \
-                     factor);
+                     rows, cols, ld, batch_x, tall, part, parts, d, t, t2,  \
+                     g, poly, factor);
   BY_TYPE(dtype, CALL)
 #undef CALL
 }

@@ -84,15 +84,10 @@ template <int N> struct Count { static constexpr int value = N; };
 // integers and v4f for 16-bit floats. STAGES steps fit in LDS, all but one of
 // them on their way.
 //
-// Measured (us for one step of one tile on each of the 256 CUs, from products
-// of 4096^2 and 2048^2 outputs): 256 x 256 by 8 waves 1.75, 128 x 128 by 8
-// waves 0.58, 64 x 64 by 4 waves 0.22 (0.36 where a CU has no second
-// workgroup). So for the same output 256 x 256 tiles take 3/4 of the time of
-// 128 x 128 ones and half of that of 64 x 64 ones, as long as they fill the
-// chip; tile_size weighs that. At 4096^3 a product of fp16 runs at 1.2
-// PFLOP/s and one of int8 at 2.6 POP/s (the library: 1.1 and 2.05). At that
-// point the matrix cores are busy 60% of the time at a clock that the power
-// limit holds at 1.75 GHz; LDS is at a quarter of its rate.
+// At 4096^3 a product of fp16 runs at 1.2 PFLOP/s and one of int8 at 2.6 POP/s
+// (the library: 1.1 and 2.05). There the matrix cores are busy 60% of the time
+// at a clock that the power limit holds at 1.75 GHz; LDS is at a quarter of
+// its rate.
 template <class ACC, int BM, int BN, int WM, int WN, int STAGES>
 struct Tile {
   static constexpr int kWaves = (BM / WM) * (BN / WN);
@@ -276,17 +271,46 @@ struct Tile {
   }
 };
 
-// The tile that needs the least time for the outputs of one launch: time for
-// a round of one tile on each CU, times the rounds.
-inline int tile_size(long m, long n, long batch, bool symmetric) {
-  auto rounds = [&](long size) {
-    const long tm = (m + size - 1) / size, tn = (n + size - 1) / size;
-    const long tiles = batch * (symmetric ? tm * (tm + 1) / 2 : tm * tn);
-    return (double)((tiles + 255) / 256);
-  };
-  const double t256 = 1.75 * rounds(256), t128 = 0.58 * rounds(128);
-  const double t64 = rounds(64) > 1 ? 0.22 * rounds(64) : 0.36;
-  return t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+// Sizes of square tiles, and what a step takes (us, fp16 and int8 alike, from
+// products of 256^2 to 4096^2 outputs): as long as a CU has one tile at most,
+// and for each further tile that a CU gets. Large tiles read less for what
+// they compute, small ones leave less of the chip idle.
+struct TileCost {
+  int size;
+  double first, more;
+};
+constexpr TileCost kTiles[] = {{256, 1.75, 1.75}, {192, 1.0, 1.1},
+                               {128, 0.6, 0.57},  {96, 0.44, 0.37},
+                               {64, 0.33, 0.21},  {32, 0.2, 0.1}};
+
+// us for one step of `tiles` tiles
+inline double step_time(const TileCost& c, long tiles) {
+  const double rounds = (double)((tiles + 255) / 256);
+  return rounds <= 1 ? c.first : c.more * rounds > c.first ? c.more * rounds
+                                                            : c.first;
 }
+
+// LAUNCH(BM, WM, WN, STAGES) with the waves' tiles and the stages for `size`.
+// Up to 128, where a CU gets one tile at most (`alone`), four steps in LDS are
+// quicker (2048^2 outputs by 128: 39 us for 64 steps, with two 47), otherwise
+// two, so that several workgroups fit (4096^2 by 128: 144 us, with four 159).
+#define BY_TILE_SIZE(size, alone, LAUNCH)          \
+  switch (size) {                                  \
+    case 256: LAUNCH(256, 128, 64, 2); break;      \
+    case 192: LAUNCH(192, 96, 48, 3); break;       \
+    case 128:                                      \
+      if (alone) LAUNCH(128, 64, 32, 4);           \
+      else LAUNCH(128, 64, 32, 2);                 \
+      break;                                       \
+    case 96:                                       \
+      if (alone) LAUNCH(96, 48, 48, 4);            \
+      else LAUNCH(96, 48, 48, 2);                  \
+      break;                                       \
+    case 64:                                       \
+      if (alone) LAUNCH(64, 32, 32, 4);            \
+      else LAUNCH(64, 32, 32, 2);                  \
+      break;                                       \
+    default: LAUNCH(32, 16, 16, 4);                \
+  }
 
 }  // namespace tile_product

@@ -361,6 +361,26 @@ def test_gpu_product_types(m, n, k, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(80, 90, 1000), (700, 900, 300),
+                                   (1000, 1100, 20000), (1500, 1530, 390),
+                                   (2040, 2047, 513), (2870, 2800, 333),
+                                   (4090, 4095, 1100), (66, 9000, 7000),
+                                   (9001, 65, 127), (30000, 300, 100)])
+def test_gpu_product_tiles(m, n, k):
+    # on the device: float64 holds the sums, so the results differ by the
+    # four roundings in float32 alone
+    g = torch.Generator(device="cuda").manual_seed(m)
+    xq, wq = (torch.randint(-128, 128, s, generator=g, device="cuda"
+                            ).to(torch.int8) for s in ((m, k), (n, k)))
+    xs, ws, b = (torch.rand(s, generator=g, device="cuda")
+                 for s in (m, n, n))
+    want, size = _product_expected(xq, xs, wq, ws, b)
+    got = ops.int8_matmul(xq, xs, wq, ws, b).double()
+    half = torch.finfo(torch.float32).eps / 2
+    assert ((got - want).abs() <= 4 * half * size * (1 + 8 * half)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [3, 90])
 def test_gpu_product_rows_that_are_not_aligned(m):
     for k in (31, 100, 256):

@@ -44,7 +44,7 @@ def _iterate(x, dtype, steps=5, c=COEFFICIENTS):
 
 
 def _far(got, want):
-    got, want = got.cpu().double(), want.double()
+    got, want = got.cpu().double(), want.cpu().double()
     return ((got - want).norm() / want.norm()).item()
 
 
@@ -231,6 +231,19 @@ def test_gpu_gram_way(shape, dtype):
                                    (1023, 400), (640, 640)])
 def test_gpu_products(shape, dtype):
     _check(_matrix(*shape, dtype=dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1030, 1300), (1500, 1530), (2050, 1950),
+                                   (2600, 2700), (4, 900, 4090),
+                                   (4, 1027, 4001), (4000, 4090)])
+def test_gpu_large(shape, dtype):
+    # one for each size of tile; on the device, or the oracle takes minutes
+    x = _matrix(*shape, dtype=dtype).cuda()
+    want = _iterate(x, torch.float64)
+    far = _far(ops.newton_schulz(x), want)
+    assert far <= _allowed(x, dtype, False), far
 
 
 @pytest.mark.gpu
