@@ -20,7 +20,7 @@ void launch_factor(const double*, int, int, double, double, double, int,
 void launch_apply(const void*, int, int, long, int, long, long, int,
                   const double*, void*, long, long, hipStream_t);
 void launch_split(const void*, int, int, int, long, long, int, double*, int,
-                  Halves, Halves, Halves, Halves, Halves, float*,
+                  Halves, Halves, Halves, Halves, Halves, Halves, float*,
                   hipStream_t);
 void launch_step(Halves, int, Halves, int, int, int, Step, int, int,
                  hipStream_t);
@@ -113,12 +113,12 @@ int shift_for(double most) {
 
 double pow2(int e) { return std::ldexp(1.0, e); }
 
-// The largest |b l + c l^2| for 0 <= l <= top.
-double largest_of_b(double b, double c, double top) {
-  double most = std::abs(b * top + c * top * top);
+// The largest |a + b l + c l^2| for 0 <= l <= top.
+double largest_of_poly(double a, double b, double c, double top) {
+  double most = std::max(std::abs(a), std::abs(a + top * (b + c * top)));
   if (c != 0) {
     const double l = -b / (2 * c);
-    if (l > 0 && l < top) most = std::max(most, std::abs(b * l + c * l * l));
+    if (l > 0 && l < top) most = std::max(most, std::abs(a + l * (b + c * l)));
   }
   return most;
 }
@@ -146,48 +146,56 @@ double largest_of_step(double a, double b, double c, double top) {
   return most;
 }
 
-// How many of the three products hi hi, hi lo, lo hi a matrix product takes.
+// How many of the three products hi hi, hi lo, lo hi a matrix product takes:
+// G = X X^T, G^2, and P X with P = a + b G + c G^2.
+//
 // float32 and float16 results take all three everywhere: about 2^-22 for each
-// product. A bfloat16 result is rounded to 2^-9, and there one product is
-// enough for G and G^2, whose rounding in 11 bits acts on large and small
-// singular values alike. The product with X needs X itself in full (an error
-// in a large singular direction that leaks into a small one is raised with it
-// by a in every later step), except in the last step, which nothing follows.
-// On gradient-like matrices (a few strong directions over noise) that leaves
-// an error of 3e-4 to 1.6e-3 of the norm before the result's own rounding
-// (1.7e-3); a single product everywhere left 4e-3 to 2e-2.
+// product, which is float32's precision within a factor of 4. A bfloat16
+// result is rounded to 2^-9, and can do with less: hi hi for G; for P X
+// hi hi + hi lo, as an error in a large singular direction that leaks into a
+// small one is raised with it by a in every later step, but hi hi in the last
+// step, which nothing follows, and in the first, as fp16 holds a bfloat16
+// input; for G^2 hi hi, and in the last two steps, where the singular values
+// are large, hi hi + 2 hi lo (G and its lo nearly commute; lo is kept twice
+// as large for that). On gradient-like and Gaussian matrices that leaves an
+// error of 0.5e-3 to 1.3e-3 of the norm before the result's own rounding
+// (1.7e-3). hi hi everywhere left 4e-3 to 2e-2, and hi hi for G^2 throughout
+// 2.2e-3 on matrices whose singular values are all alike.
 struct Precision {
-  int gram, square, step, first, last;
+  int gram, square, square_late, step, first, last;
+  float gain;
 };
 
 torch::Tensor by_products(const Matrices& v, int steps, double a, double b,
                           double c) {
-  const Precision precise = {3, 3, 3, 3, 3}, brief = {1, 1, 2, 1, 1};
+  const Precision precise = {3, 3, 3, 3, 3, 3, 1};
+  const Precision brief = {1, 1, 2, 2, 1, 1, 2};
   const Precision& p = v.type == 2 ? brief : precise;
   const long n = v.n, m = v.length, batch = v.batch;
   const long np = (n + 63) / 64 * 64, mp = (m + 63) / 64 * 64;
   TORCH_CHECK(m <= (1L << 23), "the longer side may have at most 2^23 values "
               "where the shorter one has more than ", kGramMost);
   const auto halves = v.x.options().dtype(torch::kFloat16);
-  auto matrix = [&](std::vector<torch::Tensor>& keep, long rows, long ld) {
-    keep.push_back(torch::empty({2, batch, rows, ld}, halves));
-    auto* hi = (unsigned short*)keep.back().data_ptr();
-    return Halves{hi, hi + batch * rows * ld, ld, rows * ld};
-  };
   std::vector<torch::Tensor> keep;
-  const Halves x = matrix(keep, n, mp);
-  Halves xt = matrix(keep, m, np), xt_next = matrix(keep, m, np);
-  const Halves g = matrix(keep, n, np);
-  Halves poly = matrix(keep, n, np);
-  if (p.step < 3) poly.lo = nullptr;
+  auto matrix = [&](long rows, long ld, bool lo) {
+    keep.push_back(torch::empty({lo ? 2 : 1, batch, rows, ld}, halves));
+    auto* hi = (unsigned short*)keep.back().data_ptr();
+    return Halves{hi, lo ? hi + batch * rows * ld : nullptr, ld, rows * ld};
+  };
+  const Halves x = matrix(n, mp, p.gram == 3);
+  Halves xt = matrix(m, np, true), xt_next = matrix(m, np, true);
+  const Halves g = matrix(n, np, true);
+  const Halves poly = matrix(n, np, p.step == 3);
   const int parts = 256;
   auto squares = torch::empty({batch, parts}, doubles(v.x));
   auto factor = torch::empty({batch}, v.x.options().dtype(torch::kFloat32));
   auto out = torch::empty(v.x.sizes(), v.x.options());
   const auto st = stream_of(v.x);
+  Halves xt_first = xt;
+  if (p.first == 1) xt_first.lo = nullptr;
   launch_split(v.x.data_ptr(), v.type, (int)v.rows, (int)v.cols, v.ld,
-               v.stride, (int)batch, squares.data_ptr<double>(), parts, x, xt,
-               xt_next, g, poly, factor.data_ptr<float>(), st);
+               v.stride, (int)batch, squares.data_ptr<double>(), parts, x,
+               xt_first, xt, xt_next, g, poly, factor.data_ptr<float>(), st);
 
   double bound = 1.0;  // of the singular values of X
   int ex = 14;         // stored values are 2^ex times the true ones
@@ -195,7 +203,7 @@ torch::Tensor by_products(const Matrices& v, int steps, double a, double b,
     const bool last = k + 1 == steps;
     const double top = bound * bound * 1.01;
     const int eg = shift_for(top);
-    const int ep = shift_for(largest_of_b(b, c, top) * 1.01);
+    const int ep = shift_for(largest_of_poly(a, b, c, top) * 1.01);
     bound = largest_of_step(a, b, c, bound * 1.005) * 1.01;
     // float32 holds the values in between up to here with room to spare
     TORCH_CHECK(bound < 1e12, "the coefficients let the iteration diverge");
@@ -204,6 +212,7 @@ torch::Tensor by_products(const Matrices& v, int steps, double a, double b,
 
     Step s = {};
     s.factor = factor.data_ptr<float>();
+    s.gain = p.gain;
     s.d = s.t = g;
     s.alpha = (float)pow2(eg - 2 * ex);
     s.power = k == 0 ? 2 : 0;
@@ -214,15 +223,17 @@ torch::Tensor by_products(const Matrices& v, int steps, double a, double b,
     s.e = g;
     s.alpha = (float)(c * pow2(ep - 2 * eg));
     s.beta = (float)(b * pow2(ep - eg));
+    s.diagonal = (float)(a * pow2(ep));
     s.power = 0;
-    launch_step(g, (int)n, g, (int)n, (int)n, p.square, s, (int)batch, 0, st);
+    launch_step(g, (int)n, g, (int)n, (int)n,
+                k + 2 < steps ? p.square : p.square_late, s, (int)batch, 0,
+                st);
 
     s = Step{};
     s.factor = factor.data_ptr<float>();
+    s.gain = 1;
     s.power = k == 0 ? 1 : 0;
-    s.e = x;
     s.alpha = (float)pow2(next - ep - ex);
-    s.beta = (float)(a * pow2(next - ex));
     if (last) {
       s.out = out.data_ptr();
       s.ld_out = v.cols;

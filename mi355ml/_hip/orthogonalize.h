@@ -9,14 +9,16 @@ struct Halves {
   long ld, batch;  // in values
 };
 
-// What a product is made into: v = (alpha C + beta E) factor^power.
+// What a product C is made into: v = alpha factor^power C + beta E +
+// diagonal I.
 struct Step {
-  Halves e;          // E; hi null: none
+  Halves e;          // E; hi null: neither it nor the diagonal
   Halves d, t;       // v as halves, and its transpose; hi null: not wanted
   void* out;         // or v in the type of the result
   long ld_out, batch_out;
   int tall;          // the result holds the transpose of v
-  float alpha, beta;
+  float alpha, beta, diagonal;
+  float gain;        // lo is stored, and E's is, times this
   const float* factor;  // a value for each matrix of the batch
   int power;
   int symmetric;     // v is, and its lower tiles are computed alone

@@ -53,6 +53,19 @@ template <class T> struct Four {
   struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[4]; };
 };
 
+// Four values side by side, zeros from the n-th on.
+template <class T>
+__device__ __forceinline__ void load4(const T* p, long n, float (&v)[4]) {
+  if (n >= 4) {
+    const auto raw = *(const typename Four<T>::Raw*)p;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = (float)raw.v[u];
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = u < n ? (float)p[u] : 0.0f;
+  }
+}
+
 // Element (p, q) of a panel stands at p * sp + q * sq: p counts the longer
 // side, q the shorter one. WIDE: sp is 1, otherwise sq is.
 template <class T, bool WIDE>
@@ -388,11 +401,15 @@ __global__ __launch_bounds__(256) void squares_k(
   __shared__ double sum[4];
   x += blockIdx.y * batch_x;
   double v = 0.0;
-  for (int r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int k = threadIdx.x; k < cols; k += 256) {
-      const double e = (double)(float)x[r * ld + k];
-      v += e * e;
+  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    const T* row = x + r * ld;
+    for (int k = threadIdx.x * 4; k < cols; k += 1024) {
+      float e[4];
+      load4(row + k, cols - k, e);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v += (double)e[u] * (double)e[u];
     }
+  }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
   if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = v;
@@ -404,12 +421,15 @@ __global__ __launch_bounds__(256) void squares_k(
 
 // X as fp16 numbers of magnitude up to 2^14, along both sides: [n][ld_d] and
 // [m][ld_t], filled up with zeros. X_0 = 2^-14 factor * what is stored; the
-// power of two in between is exact, the factor goes into the first step.
+// power of two in between is exact, the factor goes into the first step. The
+// filling of the buffers that later steps write is made zero here: t_later is
+// t with a lo that is not written now.
 template <class T>
 __global__ __launch_bounds__(256) void split_k(
     const T* __restrict__ x, int rows, int cols, long ld, long batch_x,
     int tall, const double* __restrict__ part, int parts, Halves d, Halves t,
-    Halves t2, Halves g, Halves poly, float* __restrict__ factor) {
+    Halves t_later, Halves t2, Halves g, Halves poly,
+    float* __restrict__ factor) {
   __shared__ float tile[64][65];
   __shared__ double sum[4];
   const int lane = threadIdx.x & 63;
@@ -439,6 +459,7 @@ __global__ __launch_bounds__(256) void split_k(
     }
   };
   const int n = tall ? cols : rows, m = tall ? rows : cols;
+  if (!t.lo) clear(t_later, m, n);
   clear(t2, m, n);
   clear(g, n, n);
   clear(poly, n, n);
@@ -447,10 +468,14 @@ __global__ __launch_bounds__(256) void split_k(
   const int across_tiles = (cols + 63) / 64;
   const int r0 = blockIdx.x / across_tiles * 64;
   const int c0 = blockIdx.x % across_tiles * 64;
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    const int r = r0 + (i >> 6), k = c0 + (i & 63);
-    const float y = r < rows && k < cols ? (float)x[r * ld + k] : 0.0f;
-    tile[i >> 6][i & 63] = fine ? ldexpf(y, 14 - e) : 0.0f;
+#pragma unroll
+  for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+    const int r = i >> 4, k = (i & 15) * 4;
+    float y[4] = {0, 0, 0, 0};
+    if (r0 + r < rows) load4(x + (r0 + r) * ld + c0 + k, cols - c0 - k, y);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      tile[r][k + u] = fine ? ldexpf(y[u], 14 - e) : 0.0f;
   }
   __syncthreads();
   const Halves along = tall ? t : d, across = tall ? d : t;
@@ -476,7 +501,7 @@ __global__ __launch_bounds__(256) void split_k(
 }
 
 // One product of a step, C = A B^T by tiles, then
-//   v = (alpha C + beta E) factor^power
+//   v = alpha factor^power C + beta E + diagonal I
 // either as halves, along both sides (for a symmetric result both are the
 // same matrix, and only its lower tiles are computed), or in the type of the
 // result.
@@ -501,12 +526,9 @@ __global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void step_k(
   const int wn0 = tj * BM + wave % (BM / WN) * WN;
   const int c = lane & 15, h = lane >> 4;
   const int rows = s.rows_a, cols = s.rows_b;
-  float alpha = p.alpha, beta = p.beta;
-  if (p.power) {
-    const float f = p.power == 2 ? p.factor[z] * p.factor[z] : p.factor[z];
-    alpha *= f;
-    beta *= f;
-  }
+  float alpha = p.alpha;
+  if (p.power) alpha *= p.factor[z];
+  if (p.power == 2) alpha *= p.factor[z];
   // the wave's own piece of LDS: 16 columns of its part, for storing along
   // the other side
   constexpr int LD = WM + 8;
@@ -525,11 +547,12 @@ __global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void step_k(
       if (p.e.hi && m < rows && n < cols) {
         const long at = z * p.e.batch + (long)m * p.e.ld + n;
         const v4h eh = *(const v4h*)(p.e.hi + at);
-        v4h el = {0, 0, 0, 0};
-        if (p.e.lo) el = *(const v4h*)(p.e.lo + at);
+        const v4h el = *(const v4h*)(p.e.lo + at);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          v[r] += beta * ((float)eh[r] + (float)el[r]);
+        for (int r = 0; r < 4; ++r) {
+          v[r] += p.beta * ((float)eh[r] + (float)el[r] / p.gain);
+          if (m == n + r) v[r] += p.diagonal;
+        }
       }
       if (OUT == kHalves) {
         v4h hi, lo;
@@ -538,7 +561,7 @@ __global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void step_k(
           // rows and columns that are not there count as zeros later
           if (m >= rows || n + r >= cols) v[r] = 0.0f;
           hi[r] = (_Float16)v[r];
-          lo[r] = (_Float16)(v[r] - (float)hi[r]);
+          lo[r] = (_Float16)((v[r] - (float)hi[r]) * p.gain);
         }
         if (p.d.hi && m < rows && n < cols) {
           const long at = z * p.d.batch + (long)m * p.d.ld + n;
@@ -729,8 +752,8 @@ extern "C" void launch_apply(const void* x, int dtype, int wide, long length,
 
 extern "C" void launch_split(const void* x, int dtype, int rows, int cols,
                              long ld, long batch_x, int batch, double* part,
-                             int parts, Halves d, Halves t, Halves t2,
-                             Halves g, Halves poly, float* factor,
+                             int parts, Halves d, Halves t, Halves t_later,
+                             Halves t2, Halves g, Halves poly, float* factor,
                              hipStream_t st) {
   const int tall = rows > cols;
   const dim3 grid(((cols + 63) / 64) * ((rows + 63) / 64), batch);
@@ -738,8 +761,8 @@ extern "C" void launch_split(const void* x, int dtype, int rows, int cols,
   hipLaunchKernelGGL((squares_k<T>), dim3(parts, batch), dim3(256), 0, st,  \
                      (const T*)x, rows, cols, ld, batch_x, part);           \
   hipLaunchKernelGGL((split_k<T>), grid, dim3(256), 0, st, (const T*)x,     \
-                     rows, cols, ld, batch_x, tall, part, parts, d, t, t2,  \
-                     g, poly, factor);
+                     rows, cols, ld, batch_x, tall, part, parts, d, t,      \
+                     t_later, t2, g, poly, factor);
   BY_TYPE(dtype, CALL)
 #undef CALL
 }
