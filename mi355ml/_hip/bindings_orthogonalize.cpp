@@ -19,6 +19,9 @@ void launch_factor(const double*, int, int, double, double, double, int,
                    double*, hipStream_t);
 void launch_apply(const void*, int, int, long, int, long, long, int,
                   const double*, void*, long, long, hipStream_t);
+int small_enough(long, int);
+void launch_small(const void*, int, int, long, int, long, long, int, int,
+                  double, double, double, void*, long, long, hipStream_t);
 void launch_split(const void*, int, int, int, long, long, int, double*, int,
                   Halves, Halves, Halves, Halves, Halves, Halves, float*,
                   hipStream_t);
@@ -264,6 +267,13 @@ torch::Tensor newton_schulz(torch::Tensor x, long steps, double a, double b,
   const c10::DeviceGuard guard(x.device());
   const Matrices v = matrices_of(x);
   if (x.numel() == 0) return torch::empty(x.sizes(), x.options());
+  if (small_enough(v.length, v.n)) {
+    auto out = torch::empty(v.x.sizes(), v.x.options());
+    launch_small(v.x.data_ptr(), v.type, v.wide, v.length, v.n, v.ld,
+                 v.stride, (int)v.batch, (int)steps, a, b, c, out.data_ptr(),
+                 v.cols, v.rows * v.cols, stream_of(v.x));
+    return out;
+  }
   if (v.n <= kGramMost)
     return apply_to(v, factor_of(gram_of(v), v.n, steps, a, b, c));
   return by_products(v, (int)steps, a, b, c);

@@ -269,11 +269,12 @@ __device__ __forceinline__ void store4(const Scales& e, long m, long n,
 }
 
 // `slab` not null: the sums of this split of K, for joining later.
-template <class T, int BM, int WM, int WN, int STAGES>
-__global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void int8_tile_k(
+template <class T, int BM, int WM, int WN, int STAGES, int GROUPS>
+__global__ __launch_bounds__(GROUPS * (BM / WM) * (BM / WN) * 64)
+void int8_tile_k(
     Sources s, Scales e, int tm, int tn, int per, int* __restrict__ slab) {
   constexpr int BN = BM;
-  typedef Tile<v4i, BM, BN, WM, WN, STAGES> P;
+  typedef Tile<v4i, BM, BN, WM, WN, STAGES, GROUPS> P;
   __shared__ __attribute__((aligned(16))) char lds[P::kLds];
   int ti, tj;
   banded(xcd_contiguous(blockIdx.x, gridDim.x), tm, tn, ti, tj);
@@ -281,9 +282,11 @@ __global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void int8_tile_k(
   const int first = blockIdx.y * per, last = min(steps, first + per);
   v4i acc[P::MI][P::NJ];
   P::run(s, ti * BM, tj * BN, 0, first, last, lds, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m0 = ti * BM + wave / (BN / WN) * WM + (lane & 15);
-  const int n0 = tj * BN + wave % (BN / WN) * WN + (lane >> 4) * 4;
+  int wm, wn;
+  if (P::place(wm, wn)) return;
+  const int lane = threadIdx.x & 63;
+  const int m0 = ti * BM + wm + (lane & 15);
+  const int n0 = tj * BN + wn + (lane >> 4) * 4;
 #pragma unroll
   for (int i = 0; i < P::MI; ++i) {
     const long m = m0 + i * 16;
@@ -430,10 +433,10 @@ void product(const Sources& s, const Scales& e, const Plan& p, int* slab,
 #define FEW(MT)                                                           \
   hipLaunchKernelGGL((int8_few_rows_k<T, MT>), grid, dim3(256), 0, st, s, \
                      e, p.per, slab)
-#define TILE(BM, WM, WN, STAGES)                                          \
-  hipLaunchKernelGGL((int8_tile_k<T, BM, WM, WN, STAGES>), grid,          \
-                     dim3((BM / WM) * (BM / WN) * 64), 0, st, s, e, p.tm, \
-                     p.tn, p.per, slab)
+#define TILE(BM, WM, WN, STAGES, GROUPS)                                 \
+  hipLaunchKernelGGL((int8_tile_k<T, BM, WM, WN, STAGES, GROUPS>), grid, \
+                     dim3(GROUPS * (BM / WM) * (BM / WN) * 64), 0, st,   \
+                     s, e, p.tm, p.tn, p.per, slab)
   if (p.rows == 16) FEW(1);
   else if (p.rows == 32) FEW(2);
   else if (p.rows == 64) FEW(4);

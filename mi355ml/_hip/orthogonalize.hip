@@ -80,62 +80,44 @@ struct Panel {
 };
 
 // ---------------------------------------------------------------------------
-// G = X X^T in 64 bits, the upper tiles of it, for n <= 16 NT.
+// n <= 128: G = X X^T in 64 bits, the upper tiles of it, for n <= 16 NT.
 // A wave takes 16 positions of the longer side at a time and has all tiles in
-// registers; the workgroup's waves are added up in order, and so are the
-// workgroups (gram_join_k): the same bits on every run.
+// registers, the next 16 positions on their way.
 // ---------------------------------------------------------------------------
-//
-// 8 waves, or 4 from 7 tiles a side on: their 28 and 36 tiles need more than
-// the 256 registers that a wave of 8 can have.
-// ---------------------------------------------------------------------------
-__host__ __device__ constexpr int gram_waves(int nt) {
-  return nt < 7 ? 8 : 4;
+template <class T, int NT, bool WIDE>
+__device__ __forceinline__ void load_group(const Panel<T, WIDE>& panel, long g,
+                                           float (&v)[4][NT]) {
+  const int c = threadIdx.x & 15, h = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int q = i * 16 + c;
+    if (WIDE) {
+      // the sum over the longer side may take it in any order: four
+      // positions side by side for a lane
+      const long p = g * 16 + h * 4;
+      float e[4] = {0, 0, 0, 0};
+      if (q < panel.n) load4(panel.x + q * panel.ld + p, panel.length - p, e);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) v[t][i] = e[t];
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) v[t][i] = panel.at(g * 16 + t * 4 + h, q);
+    }
+  }
 }
 
-template <class T, int NT, bool WIDE>
-__global__ __launch_bounds__(gram_waves(NT) * 64) void gram_k(
-    const T* __restrict__ x, long length, int n, long ld, long batch_x,
-    double* __restrict__ slab) {
-  constexpr int TILES = NT * (NT + 1) / 2, WAVES = gram_waves(NT);
-  __shared__ double sum[TILES * 256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = lane & 15, h = lane >> 4;
-  const Panel<T, WIDE> panel = {x + blockIdx.y * batch_x, length, ld, n};
-  v4d acc[TILES];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) acc[t] = v4d{0, 0, 0, 0};
-  const long groups = (length + 15) / 16;
-  const long stride = (long)gridDim.x * WAVES;
-  long g = (long)blockIdx.x * WAVES + wave;
+// Tiles FROM to FROM + COUNT of groups first, first + stride, ... added to
+// acc; AHEAD: with the next group on its way.
+template <class T, int NT, bool WIDE, int FROM, int COUNT, bool AHEAD>
+__device__ __forceinline__ void add_groups(const Panel<T, WIDE>& panel,
+                                           long first, long stride,
+                                           v4d (&acc)[COUNT]) {
+  const long groups = (panel.length + 15) / 16;
   float now[4][NT], next[4][NT];
-  auto load = [&](long g, float (&v)[4][NT]) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int q = i * 16 + c;
-      if (WIDE) {
-        // the sum over the longer side may take it in any order: four
-        // positions side by side for a lane
-        const long p = g * 16 + h * 4;
-        if (p + 4 <= length && q < n) {
-          const auto raw =
-              *(const typename Four<T>::Raw*)(panel.x + q * ld + p);
-#pragma unroll
-          for (int t = 0; t < 4; ++t) v[t][i] = (float)raw.v[t];
-        } else {
-#pragma unroll
-          for (int t = 0; t < 4; ++t) v[t][i] = panel.at(p + t, q);
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          v[t][i] = panel.at(g * 16 + t * 4 + h, q);
-      }
-    }
-  };
-  if (g < groups) load(g, now);
+  long g = first;
+  if (g < groups) load_group(panel, g, now);
   for (; g < groups; g += stride) {
-    if (g + stride < groups) load(g + stride, next);
+    if (AHEAD && g + stride < groups) load_group(panel, g + stride, next);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       double v[NT];
@@ -144,248 +126,395 @@ __global__ __launch_bounds__(gram_waves(NT) * 64) void gram_k(
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int j = i; j < NT; ++j)
-          acc[upper(NT, i, j)] = mma64(v[i], v[j], acc[upper(NT, i, j)]);
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = 0; i < NT; ++i) now[t][i] = next[t][i];
-  }
-  for (int w = 0; w < WAVES; ++w) {
-    if (wave == w) {
-#pragma unroll
-      for (int t = 0; t < TILES; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          double* to = &sum[t * 256 + (4 * i + h) * 16 + c];
-          *to = w ? *to + acc[t][i] : acc[t][i];
+        for (int j = i; j < NT; ++j) {
+          constexpr int LAST = FROM + COUNT;
+          const int k = upper(NT, i, j);
+          if (k >= FROM && k < LAST)
+            acc[k - FROM] = mma64(v[i], v[j], acc[k - FROM]);
         }
     }
-    __syncthreads();
+    if (AHEAD) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) now[t][i] = next[t][i];
+    } else if (g + stride < groups) {
+      load_group(panel, g + stride, now);
+    }
   }
+}
+
+// One wave's tiles into sum[tile * SIZE + row * LD + column].
+template <int SIZE, int LD, int COUNT>
+__device__ __forceinline__ void add_tiles(const v4d (&acc)[COUNT],
+                                          double* sum, bool begin) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int t = 0; t < COUNT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      double* to = sum + t * SIZE + (4 * i + (lane >> 4)) * LD + (lane & 15);
+      *to = begin ? acc[t][i] : *to + acc[t][i];
+    }
+}
+
+// Waves of a workgroup: three for each SIMD where their tiles leave them the
+// registers. From 7 tiles a side on two waves share a group's tiles.
+__host__ __device__ constexpr int gram_waves(int nt) {
+  return nt <= 4 ? 12 : 8;
+}
+__host__ __device__ constexpr int gram_shares(int nt) {
+  return nt < 7 ? 1 : 2;
+}
+
+// The waves are added up in their order, and so are the workgroups
+// (gram_join_k): the same bits on every run.
+template <class T, int NT, bool WIDE>
+__global__ __launch_bounds__(gram_waves(NT) * 64) void gram_k(
+    const T* __restrict__ x, long length, int n, long ld, long batch_x,
+    double* __restrict__ slab) {
+  constexpr int TILES = NT * (NT + 1) / 2, WAVES = gram_waves(NT);
+  constexpr int SHARES = gram_shares(NT), MORE = (TILES + SHARES - 1) / SHARES;
+  __shared__ double sum[TILES * 256];
+  const Panel<T, WIDE> panel = {x + blockIdx.y * batch_x, length, ld, n};
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long first = (long)blockIdx.x * (WAVES / SHARES) + wave / SHARES;
+  const long stride = (long)gridDim.x * (WAVES / SHARES);
+  auto share = [&](auto from, auto count, int mine) {
+    constexpr int FROM = decltype(from)::value, COUNT = decltype(count)::value;
+    v4d acc[COUNT];
+#pragma unroll
+    for (int t = 0; t < COUNT; ++t) acc[t] = v4d{0, 0, 0, 0};
+    add_groups<T, NT, WIDE, FROM, COUNT, true>(panel, first, stride, acc);
+    for (int w = 0; w < WAVES; ++w) {
+      if (wave == w) add_tiles<256, 16>(acc, sum + FROM * 256, w == mine);
+      __syncthreads();  // WAVES times in either share
+    }
+  };
+  if (wave % SHARES == 0)
+    share(Count<0>(), Count<MORE>(), 0);
+  else
+    share(Count<(SHARES > 1 ? MORE : 0)>(),
+          Count<(SHARES > 1 ? TILES - MORE : 1)>(), 1);
   double* out = slab + ((long)blockIdx.y * gridDim.x + blockIdx.x) *
                            (TILES * 256);
-  for (int i = threadIdx.x; i < TILES * 256; i += WAVES * 64)
-    out[i] = sum[i];
+  for (int i = threadIdx.x; i < TILES * 256; i += WAVES * 64) out[i] = sum[i];
 }
 
 __global__ __launch_bounds__(1024) void gram_join_k(
     const double* __restrict__ slab, int parts, double* __restrict__ out) {
-  __shared__ double sum[4][256];
-  const int e = threadIdx.x & 255, s = threadIdx.x >> 8;
-  const long size = (long)gridDim.x * 256;
+  __shared__ double sum[16][64];
+  // 64 entries for a workgroup, 16 shares of the parts
+  const int e = threadIdx.x & 63, s = threadIdx.x >> 6;
+  const long size = (long)gridDim.x * 64;
   const double* p = slab + (long)blockIdx.y * parts * size +
-                    blockIdx.x * 256 + e;
+                    blockIdx.x * 64 + e;
   double v = 0.0;
-#pragma unroll 8
-  for (int i = s; i < parts; i += 4) v += p[i * size];
+#pragma unroll 4
+  for (int i = s; i < parts; i += 16) v += p[i * size];
   sum[s][e] = v;
   __syncthreads();
-  if (s == 0)
-    out[blockIdx.y * size + blockIdx.x * 256 + e] =
-        (sum[0][e] + sum[1][e]) + (sum[2][e] + sum[3][e]);
+  if (s == 0) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) v += sum[k][e];
+    out[blockIdx.y * size + blockIdx.x * 64 + e] = v;
+  }
 }
 
 // ---------------------------------------------------------------------------
-// Q from G_0, one workgroup for a matrix. All matrices are polynomials in
-// G_0: symmetric, and in any order under products, so only upper tiles are
+// Q from G_0, by the 16 waves of one workgroup. All matrices are polynomials
+// in G_0: symmetric, and in any order under products, so only upper tiles are
 // held and computed. Two of them fit in LDS at n = 128; what else is alive
 // (Q, and a product on its way) stays in the registers of the waves whose
-// tiles they are.
+// tiles they are. Bound by the one CU's rate of 64-bit products: 17 of them
+// for 5 steps, each of TILES * NT * 4 instructions of 64 clocks on 4 SIMDs
+// (n = 64: 2560 clocks).
 // ---------------------------------------------------------------------------
-constexpr int kFactorWaves = 8;
+constexpr int kFactorWaves = 16;
+
+template <int NT>
+struct Factor {
+  static constexpr int TILES = NT * (NT + 1) / 2, N = 16 * NT;
+  static constexpr int MINE = (TILES + kFactorWaves - 1) / kFactorWaves;
+  static constexpr int LD = 17, SIZE = 16 * LD;  // rows of 17: no conflicts
+  static constexpr int kMatrix = TILES * SIZE;
+  // for the steps two matrices, for the product with X all of Q
+  static constexpr int kLds = 2 * kMatrix > N * N ? 2 * kMatrix : N * N;
+
+  // G_0 in s (kMatrix values) -> this wave's tiles of Q, and where they are
+  static __device__ __forceinline__ void run(double* s, int n, int steps,
+                                             double a, double b, double c,
+                                             int (&ti)[MINE], int (&tj)[MINE],
+                                             v4d (&q)[MINE]) {
+    double *s0 = s, *s1 = s + kMatrix;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 15, h = lane >> 4;
+    double trace = 0.0;
+    for (int k = lane; k < n; k += 64)
+      trace += s0[upper(NT, k >> 4, k >> 4) * SIZE + (k & 15) * (LD + 1)];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) trace += __shfl_xor(trace, d);
+    __syncthreads();
+    // a matrix of zeros stays one; one that holds NaN or an infinity becomes
+    // NaN throughout
+    const bool fine = trace < INFINITY;
+    const double shrink = trace > 0.0 ? 1.0 / trace : 0.0;
+    for (int i = threadIdx.x; i < kMatrix; i += kFactorWaves * 64)
+      s0[i] = fine ? s0[i] * shrink : 0.0;
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < MINE; ++t) {
+      int k = min(wave + t * kFactorWaves, TILES - 1), i = 0;
+      while (i + 1 < NT && upper(NT, i + 1, i + 1) <= k) ++i;
+      ti[t] = i;
+      tj[t] = i + k - upper(NT, i, i);
+    }
+    auto product = [&](const double* u, const double* v, v4d (&r)[MINE]) {
+#pragma unroll
+      for (int t = 0; t < MINE; ++t) {
+        r[t] = v4d{0, 0, 0, 0};
+        if (!mine(t)) continue;
+        // more tiles a side than that, and the places would not fit the
+        // registers
+#pragma unroll(NT <= 4 ? NT : 1)
+        for (int k = 0; k < NT; ++k) {
+          const bool ua = ti[t] <= k, vb = k <= tj[t];
+          const double* pu = u + (ua ? upper(NT, ti[t], k)
+                                     : upper(NT, k, ti[t])) * SIZE +
+                             (ua ? col * LD + h : h * LD + col);
+          const double* pv = v + (vb ? upper(NT, k, tj[t])
+                                     : upper(NT, tj[t], k)) * SIZE +
+                             (vb ? h * LD + col : col * LD + h);
+          const int su = ua ? 4 : 4 * LD, sv = vb ? 4 * LD : 4;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            r[t] = mma64(pu[kk * su], pv[kk * sv], r[t]);
+        }
+      }
+    };
+    auto put = [&](double* to, const v4d (&r)[MINE]) {
+#pragma unroll
+      for (int t = 0; t < MINE; ++t)
+        if (mine(t))
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            to[upper(NT, ti[t], tj[t]) * SIZE + (4 * i + h) * LD + col] =
+                r[t][i];
+    };
+
+    v4d r[MINE], u[MINE];
+    for (int step = 0; step < steps; ++step) {
+      product(s0, s0, r);
+#pragma unroll
+      for (int t = 0; t < MINE; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const double g =
+              s0[upper(NT, ti[t], tj[t]) * SIZE + (4 * i + h) * LD + col];
+          const bool one = ti[t] == tj[t] && 4 * i + h == col;
+          r[t][i] = (one ? a : 0.0) + b * g + c * r[t][i];
+        }
+      put(s1, r);  // P
+      const bool more = step + 1 < steps;
+      if (step == 0) {
+#pragma unroll
+        for (int t = 0; t < MINE; ++t) q[t] = r[t];
+      }
+      __syncthreads();
+      if (more) product(s0, s1, u);  // G P
+      if (step > 0) {
+        __syncthreads();
+        put(s0, q);
+        __syncthreads();
+        product(s0, s1, q);
+      }
+      if (more) {
+        __syncthreads();
+        put(s0, u);
+        __syncthreads();
+        product(s0, s1, r);  // G P P
+        __syncthreads();
+        put(s0, r);
+        __syncthreads();
+      }
+    }
+    const double scale = !fine ? (double)NAN
+                               : trace > 0.0 ? 1.0 / sqrt(trace) : 0.0;
+#pragma unroll
+    for (int t = 0; t < MINE; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[t][i] *= scale;
+  }
+
+  static __device__ __forceinline__ bool mine(int t) {
+    return (int)(threadIdx.x >> 6) + t * kFactorWaves < TILES;
+  }
+
+  // Q in the order in which the matrix instruction takes it as k x column:
+  // the k of an instruction are 16 s + 4 (lane / 16) + t, so that a lane's
+  // four of them stand side by side in a tall panel.
+  static __device__ __forceinline__ int place(int k, int column) {
+    const int s = k >> 4, h = (k >> 2) & 3, t = k & 3;
+    return ((s * 4 + t) * NT + (column >> 4)) * 64 + h * 16 + (column & 15);
+  }
+
+  static __device__ __forceinline__ void store(const int (&ti)[MINE],
+                                               const int (&tj)[MINE],
+                                               const v4d (&q)[MINE],
+                                               double* out) {
+    const int col = threadIdx.x & 15, h = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int t = 0; t < MINE; ++t)
+      if (mine(t))
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int y = ti[t] * 16 + 4 * i + h, z = tj[t] * 16 + col;
+          out[place(y, z)] = q[t][i];
+          out[place(z, y)] = q[t][i];
+        }
+  }
+};
 
 template <int NT>
 __global__ __launch_bounds__(kFactorWaves * 64) void factor_k(
     const double* __restrict__ gram, int n, int steps, double a, double b,
     double c, double* __restrict__ out) {
-  constexpr int TILES = NT * (NT + 1) / 2;
-  constexpr int MINE = (TILES + kFactorWaves - 1) / kFactorWaves;
-  constexpr int LD = 17, SIZE = 16 * LD;  // rows of 17: no bank conflicts
-  __shared__ double s0[TILES * SIZE];
-  __shared__ double s1[TILES * SIZE];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = lane & 15, h = lane >> 4;
-  gram += (long)blockIdx.x * TILES * 256;
-  out += (long)blockIdx.x * (16 * NT) * (16 * NT);
-  for (int i = threadIdx.x; i < TILES * 256; i += kFactorWaves * 64)
-    s0[(i >> 8) * SIZE + ((i >> 4) & 15) * LD + (i & 15)] = gram[i];
+  typedef Factor<NT> F;
+  __shared__ double s[2 * F::kMatrix];
+  gram += (long)blockIdx.x * F::TILES * 256;
+  for (int i = threadIdx.x; i < F::TILES * 256; i += kFactorWaves * 64)
+    s[(i >> 8) * F::SIZE + ((i >> 4) & 15) * F::LD + (i & 15)] = gram[i];
   __syncthreads();
-  double trace = 0.0;
-  for (int k = lane; k < n; k += 64)
-    trace += s0[upper(NT, k >> 4, k >> 4) * SIZE + (k & 15) * (LD + 1)];
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) trace += __shfl_xor(trace, d);
-  __syncthreads();
-  // a matrix of zeros stays one; one that holds NaN or an infinity becomes
-  // NaN throughout
-  const bool fine = trace < INFINITY;
-  const double shrink = trace > 0.0 ? 1.0 / trace : 0.0;
-  for (int i = threadIdx.x; i < TILES * SIZE; i += kFactorWaves * 64)
-    s0[i] = fine ? s0[i] * shrink : 0.0;
-  __syncthreads();
-
-  int ti[MINE], tj[MINE];
-#pragma unroll
-  for (int t = 0; t < MINE; ++t) {
-    int k = wave + t * kFactorWaves, i = 0;
-    if (k >= TILES) k = TILES - 1;  // computed twice, stored once
-    while (i + 1 < NT && upper(NT, i + 1, i + 1) <= k) ++i;
-    ti[t] = i;
-    tj[t] = i + k - upper(NT, i, i);
-  }
-  auto mine = [&](int t) { return wave + t * kFactorWaves < TILES; };
-  auto product = [&](const double* u, const double* v, v4d (&r)[MINE]) {
-#pragma unroll
-    for (int t = 0; t < MINE; ++t) {
-      r[t] = v4d{0, 0, 0, 0};
-      if (!mine(t)) continue;
-      for (int k = 0; k < NT; ++k) {
-        const bool ua = ti[t] <= k, vb = k <= tj[t];
-        const double* pu = u + (ua ? upper(NT, ti[t], k)
-                                   : upper(NT, k, ti[t])) * SIZE +
-                           (ua ? col * LD + h : h * LD + col);
-        const double* pv = v + (vb ? upper(NT, k, tj[t])
-                                   : upper(NT, tj[t], k)) * SIZE +
-                           (vb ? h * LD + col : col * LD + h);
-        const int su = ua ? 4 : 4 * LD, sv = vb ? 4 * LD : 4;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          r[t] = mma64(pu[kk * su], pv[kk * sv], r[t]);
-      }
-    }
-  };
-  auto put = [&](double* s, const v4d (&r)[MINE]) {
-#pragma unroll
-    for (int t = 0; t < MINE; ++t)
-      if (mine(t))
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[upper(NT, ti[t], tj[t]) * SIZE + (4 * i + h) * LD + col] =
-              r[t][i];
-  };
-
-  v4d q[MINE], r[MINE], u[MINE];
-  for (int step = 0; step < steps; ++step) {
-    product(s0, s0, r);
-#pragma unroll
-    for (int t = 0; t < MINE; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const double g =
-            s0[upper(NT, ti[t], tj[t]) * SIZE + (4 * i + h) * LD + col];
-        const bool one = ti[t] == tj[t] && 4 * i + h == col;
-        r[t][i] = (one ? a : 0.0) + b * g + c * r[t][i];
-      }
-    put(s1, r);  // P
-    const bool more = step + 1 < steps;
-    if (step == 0) {
-#pragma unroll
-      for (int t = 0; t < MINE; ++t) q[t] = r[t];
-    }
-    __syncthreads();
-    if (more) product(s0, s1, u);  // G P
-    if (step > 0) {
-      __syncthreads();
-      put(s0, q);
-      __syncthreads();
-      product(s0, s1, q);
-    }
-    if (more) {
-      __syncthreads();
-      put(s0, u);
-      __syncthreads();
-      product(s0, s1, r);  // G P P
-      __syncthreads();
-      put(s0, r);
-      __syncthreads();
-    }
-  }
-  const double scale = !fine ? (double)NAN
-                             : trace > 0.0 ? 1.0 / sqrt(trace) : 0.0;
-#pragma unroll
-  for (int t = 0; t < MINE; ++t)
-    if (mine(t))
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int y = ti[t] * 16 + 4 * i + h, z = tj[t] * 16 + col;
-        const double v = q[t][i] * scale;
-        out[y * (16 * NT) + z] = v;
-        out[z * (16 * NT) + y] = v;
-      }
+  int ti[F::MINE], tj[F::MINE];
+  v4d q[F::MINE];
+  F::run(s, n, steps, a, b, c, ti, tj, q);
+  F::store(ti, tj, q, out + (long)blockIdx.x * F::N * F::N);
 }
 
 // ---------------------------------------------------------------------------
-// Out = Q X, 16 positions of the longer side for a wave at a time. Q lies in
-// LDS in the order in which the matrix instruction takes it. The k of an
-// instruction are chosen so that a lane's four of them stand side by side in
-// a tall panel: 16 s + 4 (lane / 16) + t.
+// Out = Q X for 16 positions of the longer side, Q in LDS as Factor::place
+// says.
 // ---------------------------------------------------------------------------
 template <class T, int NT, bool WIDE>
-__global__ __launch_bounds__(256) void apply_k(
+__device__ __forceinline__ void load_rows(const Panel<T, WIDE>& panel, long g,
+                                          float (&v)[NT][4]) {
+  const int c = threadIdx.x & 15, h = (threadIdx.x & 63) >> 4;
+  const long p = g * 16 + c;
+#pragma unroll
+  for (int s = 0; s < NT; ++s) {
+    const int q = s * 16 + h * 4;
+    if (!WIDE && p < panel.length) {
+      load4(panel.x + p * panel.ld + q, panel.n - q, v[s]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) v[s][t] = panel.at(p, q + t);
+    }
+  }
+}
+
+template <class T, int NT, bool WIDE>
+__device__ __forceinline__ void apply_rows(const double* qs,
+                                           const Panel<T, WIDE>& panel,
+                                           long g, const float (&v)[NT][4],
+                                           T* out, long ld_out) {
+  const int lane = threadIdx.x & 63, c = lane & 15, h = lane >> 4;
+  v4d acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = v4d{0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < NT; ++s)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const double w = (double)v[s][t];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const double f = qs[((s * 4 + t) * NT + j) * 64 + lane];
+        acc[j] = WIDE ? mma64(f, w, acc[j]) : mma64(w, f, acc[j]);
+      }
+      // or the compiler reads all of Q ahead, into registers that are not
+      // there
+      if (t == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T y = (T)(float)acc[j][i];
+      if (WIDE) {
+        const long p = g * 16 + c;
+        const int q = j * 16 + 4 * i + h;
+        if (q < panel.n && p < panel.length) out[q * ld_out + p] = y;
+      } else {
+        const long p = g * 16 + 4 * i + h;
+        const int q = j * 16 + c;
+        if (q < panel.n && p < panel.length) out[p * ld_out + q] = y;
+      }
+    }
+}
+
+template <class T, int NT, bool WIDE>
+__global__ __launch_bounds__(256, NT <= 4 ? 3 : 1) void apply_k(
     const T* __restrict__ x, long length, int n, long ld, long batch_x,
     const double* __restrict__ factor, T* __restrict__ out, long ld_out,
     long batch_out) {
   constexpr int N = 16 * NT;
   __shared__ double qs[N * N];
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  const int c = lane & 15, h = lane >> 4;
-  factor += (long)blockIdx.y * N * N;
-  for (int i = threadIdx.x; i < N * N; i += 256) {
-    const int l = i & 63, j = (i >> 6) % NT, st = (i >> 6) / NT;
-    const int k = (st >> 2) * 16 + (l >> 4) * 4 + (st & 3);
-    qs[i] = factor[k * N + j * 16 + (l & 15)];
-  }
-  __syncthreads();
   const Panel<T, WIDE> panel = {x + blockIdx.y * batch_x, length, ld, n};
+  factor += (long)blockIdx.y * N * N;
   out += blockIdx.y * batch_out;
   const long groups = (length + 15) / 16;
   const long stride = (long)gridDim.x * 4;
-  for (long g = (long)blockIdx.x * 4 + wave; g < groups; g += stride) {
-    const long p = g * 16 + c;
-    float v[NT][4];
-#pragma unroll
-    for (int s = 0; s < NT; ++s) {
-      const int q = s * 16 + h * 4;
-      if (!WIDE && p < length && q + 4 <= n) {
-        const auto raw = *(const typename Four<T>::Raw*)(panel.x + p * ld + q);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) v[s][t] = (float)raw.v[t];
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) v[s][t] = panel.at(p, q + t);
-      }
-    }
-    v4d acc[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j] = v4d{0, 0, 0, 0};
+  long g = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  float now[NT][4], next[NT][4];
+  if (g < groups) load_rows(panel, g, now);
+  for (int i = threadIdx.x; i < N * N; i += 256) qs[i] = factor[i];
+  __syncthreads();
+  for (; g < groups; g += stride) {
+    if (g + stride < groups) load_rows(panel, g + stride, next);
+    apply_rows<T, NT, WIDE>(qs, panel, g, now, out, ld_out);
 #pragma unroll
     for (int s = 0; s < NT; ++s)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const double w = (double)v[s][t];
+      for (int t = 0; t < 4; ++t) now[s][t] = next[s][t];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// All of it for a small matrix, in one workgroup.
+// ---------------------------------------------------------------------------
+template <class T, int NT, bool WIDE>
+__global__ __launch_bounds__(kFactorWaves * 64) void small_k(
+    const T* __restrict__ x, long length, int n, long ld, long batch_x,
+    int steps, double a, double b, double c, T* __restrict__ out, long ld_out,
+    long batch_out) {
+  typedef Factor<NT> F;
+  __shared__ double s[F::kLds];
+  const int wave = threadIdx.x >> 6;
+  const Panel<T, WIDE> panel = {x + blockIdx.x * batch_x, length, ld, n};
+  {
+    v4d acc[F::TILES];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const double f = qs[((s * 4 + t) * NT + j) * 64 + lane];
-          acc[j] = WIDE ? mma64(f, w, acc[j]) : mma64(w, f, acc[j]);
-        }
-      }
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const T y = (T)(float)acc[j][i];
-        if (WIDE) {
-          const int q = j * 16 + 4 * i + h;
-          if (q < n && p < length) out[q * ld_out + p] = y;
-        } else {
-          const long r = g * 16 + 4 * i + h;
-          const int q = j * 16 + c;
-          if (q < n && r < length) out[r * ld_out + q] = y;
-        }
-      }
+    for (int t = 0; t < F::TILES; ++t) acc[t] = v4d{0, 0, 0, 0};
+    add_groups<T, NT, WIDE, 0, F::TILES, false>(panel, wave, kFactorWaves,
+                                                acc);
+    const long groups = (length + 15) / 16;
+    for (int w = 0; w < (groups < kFactorWaves ? groups : kFactorWaves);
+         ++w) {
+      if (wave == w) add_tiles<F::SIZE, F::LD>(acc, s, w == 0);
+      __syncthreads();
+    }
+  }
+  int ti[F::MINE], tj[F::MINE];
+  v4d q[F::MINE];
+  F::run(s, n, steps, a, b, c, ti, tj, q);
+  __syncthreads();
+  F::store(ti, tj, q, s);
+  __syncthreads();
+  float v[NT][4];
+  for (long g = wave; g < (length + 15) / 16; g += kFactorWaves) {
+    load_rows(panel, g, v);
+    apply_rows<T, NT, WIDE>(s, panel, g, v, out + blockIdx.x * batch_out,
+                            ld_out);
   }
 }
 
@@ -507,10 +636,10 @@ __global__ __launch_bounds__(256) void split_k(
 // result.
 enum { kHalves, kFloat, kFp16, kBf16 };
 
-template <int OUT, int BM, int WM, int WN, int STAGES>
-__global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void step_k(
-    Sources s, Step p) {
-  typedef Tile<v4f, BM, BM, WM, WN, STAGES> P;
+template <int OUT, int BM, int WM, int WN, int STAGES, int GROUPS>
+__global__ __launch_bounds__(GROUPS * (BM / WM) * (BM / WN) * 64)
+void step_k(Sources s, Step p) {
+  typedef Tile<v4f, BM, BM, WM, WN, STAGES, GROUPS> P;
   __shared__ __attribute__((aligned(16))) char lds[P::kLds];
   int ti, tj;
   const int b = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -520,15 +649,18 @@ __global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void step_k(
   const long z = blockIdx.y;
   P::run(s, ti * BM, tj * BM, z, 0,
          s.parts * ((s.kbytes + kStep - 1) / kStep), lds, acc);
+  int wm0, wn0;
+  if (P::place(wm0, wn0)) return;
+  wm0 += ti * BM;
+  wn0 += tj * BM;
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
-  const int wm0 = ti * BM + wave / (BM / WN) * WM;
-  const int wn0 = tj * BM + wave % (BM / WN) * WN;
   const int c = lane & 15, h = lane >> 4;
   const int rows = s.rows_a, cols = s.rows_b;
   float alpha = p.alpha;
   if (p.power) alpha *= p.factor[z];
   if (p.power == 2) alpha *= p.factor[z];
+  const float ungain = 1.0f / p.gain;
   // the wave's own piece of LDS: 16 columns of its part, for storing along
   // the other side
   constexpr int LD = WM + 8;
@@ -550,7 +682,7 @@ __global__ __launch_bounds__((BM / WM) * (BM / WN) * 64) void step_k(
         const v4h el = *(const v4h*)(p.e.lo + at);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          v[r] += p.beta * ((float)eh[r] + (float)el[r] / p.gain);
+          v[r] += p.beta * ((float)eh[r] + (float)el[r] * ungain);
           if (m == n + r) v[r] += p.diagonal;
         }
       }
@@ -631,9 +763,9 @@ void step_as(Sources s, Step p, int batch, hipStream_t st) {
   p.tn = (s.rows_b + size - 1) / size;
   const bool alone = tiles_of(size) * batch <= 256;
   const dim3 grid((unsigned)tiles_of(size), batch);
-#define STEP(BM, WM, WN, STAGES)                                 \
-  hipLaunchKernelGGL((step_k<OUT, BM, WM, WN, STAGES>), grid,    \
-                     dim3((BM / WM) * (BM / WN) * 64), 0, st, s, p)
+#define STEP(BM, WM, WN, STAGES, GROUPS)                              \
+  hipLaunchKernelGGL((step_k<OUT, BM, WM, WN, STAGES, GROUPS>), grid, \
+                     dim3(GROUPS * (BM / WM) * (BM / WN) * 64), 0, st, s, p)
   BY_TILE_SIZE(size, alone, STEP)
 #undef STEP
 }
@@ -661,6 +793,19 @@ void apply_as(const T* x, bool wide, long length, int n, long ld, long bx,
   else
     hipLaunchKernelGGL((apply_k<T, NT, false>), grid, block, 0, st, x, length,
                        n, ld, bx, factor, out, ld_out, batch_out);
+}
+
+template <class T, int NT>
+void small_as(const T* x, bool wide, long length, int n, long ld, long bx,
+              int batch, int steps, double a, double b, double c, T* out,
+              long ld_out, long batch_out, hipStream_t st) {
+  const dim3 grid(batch), block(kFactorWaves * 64);
+  if (wide)
+    hipLaunchKernelGGL((small_k<T, NT, true>), grid, block, 0, st, x, length,
+                       n, ld, bx, steps, a, b, c, out, ld_out, batch_out);
+  else
+    hipLaunchKernelGGL((small_k<T, NT, false>), grid, block, 0, st, x, length,
+                       n, ld, bx, steps, a, b, c, out, ld_out, batch_out);
 }
 
 #define BY_TILES(nt, CALL) \
@@ -695,6 +840,23 @@ void apply_type(const T* x, bool wide, long length, int n, long ld, long bx,
 #undef CALL
 }
 
+// n up to 64 (more tiles than that do not fit the registers of 16 waves)
+template <class T>
+void small_type(const T* x, bool wide, long length, int n, long ld, long bx,
+                int batch, int steps, double a, double b, double c, T* out,
+                long ld_out, long batch_out, hipStream_t st) {
+#define CALL(NT)                                                            \
+  small_as<T, NT>(x, wide, length, n, ld, bx, batch, steps, a, b, c, out,   \
+                  ld_out, batch_out, st);
+  switch ((n + 15) / 16) {
+    case 1: CALL(1) break;
+    case 2: CALL(2) break;
+    case 3: CALL(3) break;
+    default: CALL(4)
+  }
+#undef CALL
+}
+
 }  // namespace
 
 #define BY_TYPE(dtype, CALL)             \
@@ -704,7 +866,8 @@ void apply_type(const T* x, bool wide, long length, int n, long ld, long bx,
 
 extern "C" int gram_parts(long length, int n, int batch) {
   const long groups = (length + 15) / 16;
-  const long each = 4 * gram_waves((n + 15) / 16);  // 4 groups for a wave
+  const int nt = (n + 15) / 16;
+  const long each = 4 * gram_waves(nt) / gram_shares(nt);  // 4 for a wave
   const long parts = (groups + each - 1) / each;
   const long most = batch < 256 ? 256 / batch : 1;
   return (int)(parts < 1 ? 1 : parts > most ? most : parts);
@@ -721,7 +884,7 @@ extern "C" void launch_gram(const void* x, int dtype, int wide, long length,
 #undef CALL
   const int nt = (n + 15) / 16;
   if (parts > 1)
-    hipLaunchKernelGGL(gram_join_k, dim3(nt * (nt + 1) / 2, batch),
+    hipLaunchKernelGGL(gram_join_k, dim3(nt * (nt + 1) * 2, batch),
                        dim3(1024), 0, st, slab, parts, gram);
 }
 
@@ -741,11 +904,31 @@ extern "C" void launch_apply(const void* x, int dtype, int wide, long length,
                              long batch_out, hipStream_t st) {
   const long groups = (length + 15) / 16;
   const long want = (groups + 15) / 16;
-  const long most = n <= 64 ? 1024 : 256;
+  const long most = n <= 64 ? 768 : 256;  // what a CU has room for
   const int blocks = (int)(want < 1 ? 1 : want > most ? most : want);
 #define CALL(T)                                                           \
   apply_type((const T*)x, wide, length, n, ld, batch_x, batch, factor,    \
              (T*)out, ld_out, batch_out, blocks, st);
+  BY_TYPE(dtype, CALL)
+#undef CALL
+}
+
+// Whether one workgroup for a matrix is quicker than three launches: as long
+// as its products with X take less than those (about 16 positions of the
+// longer side by 16 of the shorter one for each tile, 64 clocks).
+extern "C" int small_enough(long length, int n) {
+  const long nt = (n + 15) / 16, groups = (length + 15) / 16;
+  return nt <= 4 && groups * (nt * (nt + 1) / 2 + nt * nt) <= 240;
+}
+
+extern "C" void launch_small(const void* x, int dtype, int wide, long length,
+                             int n, long ld, long batch_x, int batch,
+                             int steps, double a, double b, double c,
+                             void* out, long ld_out, long batch_out,
+                             hipStream_t st) {
+#define CALL(T)                                                             \
+  small_type((const T*)x, wide, length, n, ld, batch_x, batch, steps, a, b, \
+             c, (T*)out, ld_out, batch_out, st);
   BY_TYPE(dtype, CALL)
 #undef CALL
 }

@@ -82,15 +82,21 @@ template <int N> struct Count { static constexpr int value = N; };
 
 // BM x BN: the workgroup's tile, WM x WN: a wave's. ACC is v4i for 8-bit
 // integers and v4f for 16-bit floats. STAGES steps fit in LDS, all but one of
-// them on their way.
+// them on their way. With GROUPS = 2 twice the waves share a tile: the second
+// half of them takes the second half of every step, and gives its sums to the
+// first at the end. That is for a CU's only workgroup, with one wave for each
+// SIMD otherwise (64 steps of a 64 x 64 tile 17.6 us, with one group 21.6).
 //
 // At 4096^3 a product of fp16 runs at 1.2 PFLOP/s and one of int8 at 2.6 POP/s
 // (the library: 1.1 and 2.05). There the matrix cores are busy 60% of the time
 // at a clock that the power limit holds at 1.75 GHz; LDS is at a quarter of
-// its rate.
-template <class ACC, int BM, int BN, int WM, int WN, int STAGES>
+// its rate. Small tiles are bound by what a CU takes in: a step of 64 x 64
+// is 16 KB in 520 clocks, of about 40 B a clock that loads alone reach.
+template <class ACC, int BM, int BN, int WM, int WN, int STAGES, int GROUPS>
 struct Tile {
-  static constexpr int kWaves = (BM / WM) * (BN / WN);
+  static constexpr int kCols = BN / WN;
+  static constexpr int kGroup = (BM / WM) * kCols;  // waves of a group
+  static constexpr int kWaves = GROUPS * kGroup;
   static constexpr int kThreads = kWaves * 64;
   static constexpr int MI = WM / 16, NJ = WN / 16;
   static constexpr int kStage = (BM + BN) * kStep;
@@ -116,6 +122,14 @@ struct Tile {
     __builtin_amdgcn_sched_group_barrier(0x008, M - EACH * (R + V), 0);
   }
 
+  // The wave's place in the tile. Waves of a second group are done after run.
+  static __device__ __forceinline__ int place(int& wm, int& wn) {
+    const int wave = threadIdx.x >> 6;
+    wm = wave % kGroup / kCols * WM;
+    wn = wave % kCols * WN;
+    return wave / kGroup;
+  }
+
   // acc[i][j][r] is the sum for row  m = i * 16 + lane % 16  and column
   // n = j * 16 + lane / 16 * 4 + r  of the wave's part of the tile: B goes in
   // as the first operand, so that a lane ends with four columns side by side.
@@ -125,21 +139,26 @@ struct Tile {
                                              ACC (&acc)[MI][NJ]) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / (BN / WN), wn = wave % (BN / WN);
-    constexpr int LA = BM / 8 / kWaves, LB = BN / 8 / kWaves;
+    const int group = wave / kGroup;
+    const int wm = wave % kGroup / kCols, wn = wave % kCols;
+    // the wave's share of the rows to load, 8 at a time, A's before B's
+    constexpr int LOADS = (BM + BN) / 8 / kWaves;
+    static_assert(LOADS * kWaves * 8 == BM + BN, "");
     const int r8 = lane >> 3;
     const int c16 = ((lane & 7) ^ r8) * 16;
     // rows behind the last are read from the last one; nothing is stored
     // from what they give
-    unsigned oa[LA], ob[LB];
+    unsigned at_row[LOADS];
+    bool of_a[LOADS];
 #pragma unroll
-    for (int i = 0; i < LA; ++i)
-      oa[i] = (unsigned)(min(m0 + (i * kWaves + wave) * 8 + r8,
-                             s.rows_a - 1) - m0) * s.row_a;
-#pragma unroll
-    for (int i = 0; i < LB; ++i)
-      ob[i] = (unsigned)(min(n0 + (i * kWaves + wave) * 8 + r8,
-                             s.rows_b - 1) - n0) * s.row_b;
+    for (int u = 0; u < LOADS; ++u) {
+      const int r = (u * kWaves + wave) * 8;
+      of_a[u] = r < BM;
+      at_row[u] =
+          of_a[u]
+              ? (unsigned)(min(m0 + r + r8, s.rows_a - 1) - m0) * s.row_a
+              : (unsigned)(min(n0 + r - BM + r8, s.rows_b - 1) - n0) * s.row_b;
+    }
     const int steps = (s.kbytes + kStep - 1) / kStep;
     const int tail = s.kbytes - (steps - 1) * kStep;  // bytes of the last step
     const long at_a = batch * s.batch_a + (long)m0 * s.row_a;
@@ -157,19 +176,13 @@ struct Tile {
       // a chunk that begins behind the row's end is read from the step's
       // first one instead, and masked below
       const unsigned c = kInt && k == steps - 1 && c16 >= tail ? 0 : c16;
-      char* la = lds + buf * kStage + wave * 1024;
-      char* lb = la + BM * kStep;
+      char* to = lds + buf * kStage + wave * 1024;
 #pragma unroll
-      for (int i = 0; i < LA; ++i)
+      for (int u = 0; u < LOADS; ++u)
         __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(pa + (oa[i] + c)),
-            (__attribute__((address_space(3))) void*)(la + i * kWaves * 1024),
-            16, 0, 0);
-#pragma unroll
-      for (int i = 0; i < LB; ++i)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(pb + (ob[i] + c)),
-            (__attribute__((address_space(3))) void*)(lb + i * kWaves * 1024),
+            (const __attribute__((address_space(1))) void*)(
+                (of_a[u] ? pa : pb) + (at_row[u] + c)),
+            (__attribute__((address_space(3))) void*)(to + u * kWaves * 1024),
             16, 0, 0);
       const bool wrap = ++k == steps;
       k = wrap ? 0 : k;
@@ -201,7 +214,7 @@ struct Tile {
     // All loads but the last N steps' are in, and every wave is done with
     // the buffer of the step before.
     auto turn = [&](auto n) {
-      constexpr int LEFT = decltype(n)::value * (LA + LB);
+      constexpr int LEFT = decltype(n)::value * LOADS;
       // vmcnt in bits 0-3 and 14-15, lgkmcnt 0, expcnt not waited for
       constexpr int IMM = (LEFT & 15) | ((LEFT >> 4) << 14) | (7 << 4);
       __builtin_amdgcn_sched_barrier(0);
@@ -231,42 +244,85 @@ struct Tile {
       if (u < count) load(u);
     if (count >= STAGES) turn(Count<STAGES - 1>());
     else turn(Count<0>());
-    fetch(f0, 0, 0);
+    fetch(f0, 0, group);
     int buf = 0;
     auto after = [](int b) { return b + 1 == STAGES ? 0 : b + 1; };
     int t = 0;
-    for (; t + STAGES < count; ++t) {
-      fetch(f1, buf, 1);
-      multiply(f0);
-      interleave<0>();
-      turn(Count<STAGES - 2>());
-      const int next = after(buf);
-      fetch(f0, next, 0);
-      load(buf);
-      multiply(f1);
-      interleave<LA + LB>();
-      buf = next;
-    }
-    for (; t + 1 < count; ++t) {
-      fetch(f1, buf, 1);
-      multiply(f0);
-      interleave<0>();
-      turn(Count<0>());
-      buf = after(buf);
-      fetch(f0, buf, 0);
-      multiply(f1);
-      interleave<0>();
-    }
-    fetch(f1, buf, 1);
-    if (kInt && tail < kStep && last % steps == 0) {
+    auto cut = [&](Half& f, int from) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        f0.b[j] = keep_bytes(f0.b[j], tail - (lane >> 4) * 16);
-        f1.b[j] = keep_bytes(f1.b[j], tail - 64 - (lane >> 4) * 16);
+      for (int j = 0; j < NJ; ++j)
+        f.b[j] = keep_bytes(f.b[j], tail - from - (lane >> 4) * 16);
+    };
+    const bool ragged = kInt && tail < kStep && last % steps == 0;
+    if constexpr (GROUPS == 1) {
+      for (; t + STAGES < count; ++t) {
+        fetch(f1, buf, 1);
+        multiply(f0);
+        interleave<0>();
+        turn(Count<STAGES - 2>());
+        const int next = after(buf);
+        fetch(f0, next, 0);
+        load(buf);
+        multiply(f1);
+        interleave<LOADS>();
+        buf = next;
+      }
+      for (; t + 1 < count; ++t) {
+        fetch(f1, buf, 1);
+        multiply(f0);
+        interleave<0>();
+        turn(Count<0>());
+        buf = after(buf);
+        fetch(f0, buf, 0);
+        multiply(f1);
+        interleave<0>();
+      }
+      fetch(f1, buf, 1);
+      if (ragged) {
+        cut(f0, 0);
+        cut(f1, 64);
+      }
+      multiply(f0);
+      multiply(f1);
+    } else {
+      // each group of waves has its half of every step
+      auto step = [&](Half& now, Half& next, bool more) {
+        if (more) turn(Count<STAGES - 2>());
+        else turn(Count<0>());
+        const int b = after(buf);
+        fetch(next, b, group);
+        if (more) load(buf);
+        multiply(now);
+        buf = b;
+      };
+      for (; t + STAGES + 1 < count; t += 2) {
+        step(f0, f1, true);
+        interleave<LOADS>();
+        step(f1, f0, true);
+        interleave<LOADS>();
+      }
+      for (; t + 1 < count; ++t) {
+        step(f0, f1, t + STAGES < count);
+        f0 = f1;
+      }
+      if (ragged) cut(f0, group * 64);
+      multiply(f0);
+      __syncthreads();  // the last reads of the buffers are done
+      ACC* sums = (ACC*)lds + wave % kGroup * (MI * NJ * 64) + lane;
+      if (group == 1) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) sums[(i * NJ + j) * 64] = acc[i][j];
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j] += sums[(i * NJ + j) * 64];
       }
     }
-    multiply(f0);
-    multiply(f1);
     __syncthreads();
   }
 };
@@ -280,8 +336,8 @@ struct TileCost {
   double first, more;
 };
 constexpr TileCost kTiles[] = {{256, 1.75, 1.75}, {192, 1.0, 1.1},
-                               {128, 0.6, 0.57},  {96, 0.44, 0.37},
-                               {64, 0.33, 0.21},  {32, 0.2, 0.1}};
+                               {128, 0.6, 0.57},  {96, 0.41, 0.37},
+                               {64, 0.28, 0.21},  {32, 0.2, 0.1}};
 
 // us for one step of `tiles` tiles
 inline double step_time(const TileCost& c, long tiles) {
@@ -290,27 +346,27 @@ inline double step_time(const TileCost& c, long tiles) {
                                                             : c.first;
 }
 
-// LAUNCH(BM, WM, WN, STAGES) with the waves' tiles and the stages for `size`.
-// Up to 128, where a CU gets one tile at most (`alone`), four steps in LDS are
-// quicker (2048^2 outputs by 128: 39 us for 64 steps, with two 47), otherwise
-// two, so that several workgroups fit (4096^2 by 128: 144 us, with four 159).
+// LAUNCH(BM, WM, WN, STAGES, GROUPS) for tiles of `size`. Up to 128, where a
+// CU gets one tile at most (`alone`), four steps in LDS are quicker (2048^2
+// outputs by 128: 39 us for 64 steps, with two 47), otherwise two, so that
+// several workgroups fit (4096^2 by 128: 144 us, with four 159).
 #define BY_TILE_SIZE(size, alone, LAUNCH)          \
   switch (size) {                                  \
-    case 256: LAUNCH(256, 128, 64, 2); break;      \
-    case 192: LAUNCH(192, 96, 48, 3); break;       \
+    case 256: LAUNCH(256, 128, 64, 2, 1); break;   \
+    case 192: LAUNCH(192, 96, 48, 3, 1); break;    \
     case 128:                                      \
-      if (alone) LAUNCH(128, 64, 32, 4);           \
-      else LAUNCH(128, 64, 32, 2);                 \
+      if (alone) LAUNCH(128, 64, 32, 4, 1);        \
+      else LAUNCH(128, 64, 32, 2, 1);              \
       break;                                       \
     case 96:                                       \
-      if (alone) LAUNCH(96, 48, 48, 4);            \
-      else LAUNCH(96, 48, 48, 2);                  \
+      if (alone) LAUNCH(96, 48, 48, 4, 2);         \
+      else LAUNCH(96, 48, 48, 2, 1);               \
       break;                                       \
     case 64:                                       \
-      if (alone) LAUNCH(64, 32, 32, 4);            \
-      else LAUNCH(64, 32, 32, 2);                  \
+      if (alone) LAUNCH(64, 32, 32, 4, 2);         \
+      else LAUNCH(64, 32, 32, 2, 1);               \
       break;                                       \
-    default: LAUNCH(32, 16, 16, 4);                \
+    default: LAUNCH(32, 16, 16, 4, 1);             \
   }
 
 }  // namespace tile_product
