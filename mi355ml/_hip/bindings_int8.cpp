@@ -13,6 +13,10 @@ long int8_product_workspace(long, long, long);
 void launch_int8_product(const int8_t*, long, const float*, const int8_t*,
                          long, const float*, const float*, long, long, long,
                          void*, int, int*, hipStream_t);
+int int8_linear_in_one(long, long, long);
+void launch_int8_linear(const void*, int, long, const int8_t*, long,
+                        const float*, const float*, long, long, long, void*,
+                        int, hipStream_t);
 }
 
 namespace {
@@ -71,6 +75,14 @@ torch::Tensor aligned_rows(const torch::Tensor& q) {
   return view;
 }
 
+torch::Tensor vector_of(const torch::Tensor& t, long size,
+                        const torch::Device& device, const char* name) {
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == size &&
+              t.dtype() == torch::kFloat32 && t.device() == device,
+              name, " must be float32 of ", size, " values on ", device);
+  return t.contiguous();
+}
+
 torch::Tensor int8_product(torch::Tensor xq, torch::Tensor xs,
                            torch::Tensor wq, torch::Tensor ws,
                            c10::optional<torch::Tensor> bias,
@@ -86,18 +98,12 @@ torch::Tensor int8_product(torch::Tensor xq, torch::Tensor xs,
               "32 bits (got ", k, ")");
   TORCH_CHECK(m < (1L << 31) - 256 && n < (1L << 31) - 256,
               "xq or wq has too many rows");
-  auto scale = [&](const torch::Tensor& t, long size, const char* name) {
-    TORCH_CHECK(t.dim() == 1 && t.size(0) == size &&
-                t.dtype() == torch::kFloat32 && t.device() == xq.device(),
-                name, " must be float32 of ", size, " values on xq's device");
-    return t.contiguous();
-  };
   TORCH_CHECK(wq.device() == xq.device(), "wq must be on xq's device");
   const c10::DeviceGuard guard(xq.device());
-  xs = scale(xs, m, "x_scale");
-  ws = scale(ws, n, "w_scale");
+  xs = vector_of(xs, m, xq.device(), "x_scale");
+  ws = vector_of(ws, n, xq.device(), "w_scale");
   torch::Tensor b;
-  if (bias.has_value()) b = scale(*bias, n, "bias");
+  if (bias.has_value()) b = vector_of(*bias, n, xq.device(), "bias");
   const int type = type_id(out_type);
   auto out = torch::empty({m, n}, xq.options().dtype(out_type));
   if (m == 0 || n == 0) return out;
@@ -121,6 +127,38 @@ torch::Tensor int8_product(torch::Tensor xq, torch::Tensor xs,
   return out;
 }
 
+// quantize_rows of x and its product, in one launch where x is small
+torch::Tensor int8_linear(torch::Tensor x, torch::Tensor wq, torch::Tensor ws,
+                          c10::optional<torch::Tensor> bias,
+                          torch::ScalarType out_type) {
+  TORCH_CHECK(x.is_cuda(), "x must be on the GPU");
+  TORCH_CHECK(x.dim() == 2 && wq.dim() == 2 && x.size(1) == wq.size(1),
+              "x and wq must be [m, k] and [n, k]");
+  const long m = x.size(0), n = wq.size(0), k = x.size(1);
+  if (m == 0 || n == 0 || k == 0 || !int8_linear_in_one(m, n, k)) {
+    auto [xq, xs] = quantize_rows(x);
+    return int8_product(xq, xs, wq, ws, bias, out_type);
+  }
+  TORCH_CHECK(wq.dtype() == torch::kInt8 && wq.device() == x.device(),
+              "wq must be int8 on x's device");
+  TORCH_CHECK(n < (1L << 31) - 256, "wq has too many rows");
+  const int xtype = type_id(x.scalar_type()), type = type_id(out_type);
+  const c10::DeviceGuard guard(x.device());
+  ws = vector_of(ws, n, x.device(), "w_scale");
+  torch::Tensor b;
+  if (bias.has_value()) b = vector_of(*bias, n, x.device(), "bias");
+  if (k > 1 && x.stride(1) != 1) x = x.contiguous();
+  wq = aligned_rows(wq);
+  auto out = torch::empty({m, n}, x.options().dtype(out_type));
+  launch_int8_linear(x.data_ptr(), xtype, x.stride(0),
+                     wq.data_ptr<int8_t>(),
+                     n == 1 ? (k + 15) / 16 * 16 : wq.stride(0),
+                     ws.data_ptr<float>(),
+                     b.defined() ? b.data_ptr<float>() : nullptr, m, n, k,
+                     out.data_ptr(), type, stream_of(x));
+  return out;
+}
+
 }  // namespace
 
 void register_int8(py::module_& mod) {
@@ -128,4 +166,6 @@ void register_int8(py::module_& mod) {
           "8-bit rows and the scale of each");
   mod.def("int8_product", &int8_product,
           "product of 8-bit matrices with a scale for each row and column");
+  mod.def("int8_linear", &int8_linear,
+          "quantize_rows and int8_product of its result");
 }

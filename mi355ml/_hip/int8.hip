@@ -31,17 +31,11 @@ template <> __device__ __forceinline__ float widen(__bf16 v) {
 // ---------------------------------------------------------------------------
 
 // rne(x / s) with the quotient taken exactly. x * (1 / s) is off by less than
-// one step of q next to the middle of two integers only; the remainder
+// one step of q, and next to the middle of two integers only; the remainder
 // x - q s is a multiple of s's last bit, so the fma gives it without a
-// rounding and says on which side x lies.
-__device__ __forceinline__ int nearest(float x, float s, float inv) {
-  float q = rintf(x * inv);
-  const float r = fmaf(-q, s, x);
-  const float a = fabsf(r), h = 0.5f * s;
-  const bool odd = ((int)q) & 1;
-  if (a > h || (a == h && odd)) q += copysignf(1.0f, r);
-  return (int)q;
-}
+// rounding, and it says on which side x lies. 1.5 * 2^23 added to a number
+// leaves it rounded in the low bits.
+constexpr float kLowBits = 12582912.0f;
 
 struct RowScale {
   float s, inv;
@@ -53,13 +47,40 @@ struct RowScale {
     inv = __fdiv_rn(1.0f, s);
   }
   __device__ __forceinline__ float scale() const { return fine ? s : NAN; }
-  __device__ __forceinline__ int operator()(float x) const {
+  // every case, for one value
+  __device__ __forceinline__ int slowly(float x) const {
     if (!fine || s == 0.0f) return 0;
     if (tiny) {
       const double q = rint((double)x / (double)s);
       return (int)fmin(127.0, fmax(-127.0, q));
     }
-    return nearest(x, s, inv);
+    float q = fmaf(x, inv, kLowBits) - kLowBits;
+    const float r = fmaf(-q, s, x);
+    const float a = fabsf(r), h = 0.5f * s;
+    if (a > h || (a == h && ((int)q & 1))) q += copysignf(1.0f, r);
+    return (int)q;
+  }
+  // N values to N bytes, N a multiple of 4: a product, a remainder and a
+  // maximum for a value, as long as none of them lies in the middle
+  template <int N>
+  __device__ __forceinline__ void pack(const float (&x)[N],
+                                       uint32_t (&w)[N / 4]) const {
+    uint32_t t[N];
+    float far = 0.0f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float v = fmaf(x[e], inv, kLowBits);
+      t[e] = __float_as_uint(v);
+      far = fmaxf(far, fabsf(fmaf(-(v - kLowBits), s, x[e])));
+    }
+    if (!fine || tiny || far >= 0.5f * s) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) t[e] = (uint32_t)slowly(x[e]);
+    }
+#pragma unroll
+    for (int d = 0; d < N / 4; ++d)
+      w[d] = __builtin_amdgcn_perm(t[4 * d + 1], t[4 * d], 0x0c0c0400) |
+             __builtin_amdgcn_perm(t[4 * d + 3], t[4 * d + 2], 0x04000c0c);
   }
 };
 
@@ -73,68 +94,70 @@ template <class T, int VEC> struct Chunk {
   struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[VEC]; };
 };
 
+// VEC values from the row's at-th on, zeros behind its end.
+template <class T, int VEC>
+__device__ __forceinline__ void load_chunk(const T* row, long at, long k,
+                                           float (&v)[VEC]) {
+  if (at + VEC <= k) {
+    const auto raw = *(const typename Chunk<T, VEC>::Raw*)(row + at);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = widen(raw.v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = at + e < k ? widen(row[at + e]) : 0.0f;
+  }
+}
+
 // A row for LANES lanes, each holding CH chunks of 16 bytes of it between the
-// two passes (maximum, then rounding), so that x is read once. Memory-bound:
-// a few comparisons and about ten operations for the rounding of a value,
-// against the 5 (or 3) bytes that it moves.
-template <class T, int LANES, int CH>
+// two passes (maximum, then rounding), so that x is read once; EACH rows at a
+// time for a lane, so that enough loads are on their way. Memory-bound: about
+// ten operations a value against the 5 (or 3) bytes that it moves.
+template <class T, int LANES, int CH, int EACH>
 __global__ __launch_bounds__(256) void quantize_rows_k(
     const T* __restrict__ x, long m, int k, long stride,
     int8_t* __restrict__ q, long qstride, float* __restrict__ scale) {
   constexpr int VEC = 16 / sizeof(T);
   constexpr int ROWS = 256 / LANES;
-  typedef typename Chunk<T, VEC>::Raw Raw;
   __shared__ float part[4];
   const int lane = threadIdx.x % LANES;
-  const long row = (long)blockIdx.x * ROWS + threadIdx.x / LANES;
-  const bool here = row < m;
-  const T* xr = x + (here ? row : 0) * stride;
-  float v[CH][VEC];
-  float big = 0.0f;
+  const long first = (long)blockIdx.x * (ROWS * EACH) + threadIdx.x / LANES;
+  float v[EACH][CH][VEC];
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const int at = (c * LANES + lane) * VEC;
-    if (at + VEC <= k) {
-      const Raw raw = *(const Raw*)(xr + at);
+  for (int r = 0; r < EACH; ++r) {
+    const long row = min(first + r * ROWS, m - 1);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[c][e] = widen(raw.v[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        v[c][e] = at + e < k ? widen(xr[at + e]) : 0.0f;
-    }
+    for (int c = 0; c < CH; ++c)
+      load_chunk<T, VEC>(x + row * stride, (c * LANES + lane) * VEC, k,
+                         v[r][c]);
   }
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+  for (int r = 0; r < EACH; ++r) {
+    const long row = first + r * ROWS;
+    float big = 0.0f;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) big = max_abs(big, v[c][e]);
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-  for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1)
-    big = max_abs(big, __shfl_xor(big, d));
-  if (LANES > 64) {
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = big;
-    __syncthreads();
-    big = part[0];
+      for (int e = 0; e < VEC; ++e) big = max_abs(big, v[r][c][e]);
 #pragma unroll
-    for (int w = 1; w < 4; ++w) big = max_abs(big, part[w]);
-  }
-  if (!here) return;
-  const RowScale rs(big);
-  if (lane == 0) scale[row] = rs.scale();
-  int8_t* qr = q + row * qstride;
+    for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1)
+      big = max_abs(big, __shfl_xor(big, d));
+    if (LANES > 64) {
+      if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = big;
+      __syncthreads();
+      big = part[0];
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const int at = (c * LANES + lane) * VEC;
-    uint32_t w[VEC / 4];
-#pragma unroll
-    for (int d = 0; d < VEC / 4; ++d) {
-      w[d] = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[d] |= (uint32_t)(uint8_t)(int8_t)rs(v[c][4 * d + e]) << (8 * e);
+      for (int w = 1; w < 4; ++w) big = max_abs(big, part[w]);
     }
-    // the row's last 16 bytes are filled up with zeros
-    if (at < qstride) {
+    if (row >= m) continue;
+    const RowScale rs(big);
+    if (lane == 0) scale[row] = rs.scale();
+    int8_t* qr = q + row * qstride;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int at = (c * LANES + lane) * VEC;
+      if (at >= qstride) continue;  // the last 16 bytes are filled with zeros
+      uint32_t w[VEC / 4];
+      rs.pack(v[r][c], w);
 #pragma unroll
       for (int d = 0; d < VEC / 4; ++d) ((uint32_t*)(qr + at))[d] = w[d];
     }
@@ -147,19 +170,14 @@ __global__ __launch_bounds__(256) void quantize_long_rows_k(
     const T* __restrict__ x, long m, long k, long stride,
     int8_t* __restrict__ q, long qstride, float* __restrict__ scale) {
   constexpr int VEC = 16 / sizeof(T);
-  typedef typename Chunk<T, VEC>::Raw Raw;
   __shared__ float part[4];
   const long row = blockIdx.x;
   const T* xr = x + row * stride;
-  float big = 0.0f;
+  float big = 0.0f, v[VEC];
   for (long at = (long)threadIdx.x * VEC; at < k; at += 256 * VEC) {
-    if (at + VEC <= k) {
-      const Raw raw = *(const Raw*)(xr + at);
+    load_chunk<T, VEC>(xr, at, k, v);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) big = max_abs(big, widen(raw.v[e]));
-    } else {
-      for (long e = at; e < k; ++e) big = max_abs(big, widen(xr[e]));
-    }
+    for (int e = 0; e < VEC; ++e) big = max_abs(big, v[e]);
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) big = max_abs(big, __shfl_xor(big, d));
@@ -172,29 +190,9 @@ __global__ __launch_bounds__(256) void quantize_long_rows_k(
   if (threadIdx.x == 0) scale[row] = rs.scale();
   int8_t* qr = q + row * qstride;
   for (long at = (long)threadIdx.x * VEC; at < qstride; at += 256 * VEC) {
+    load_chunk<T, VEC>(xr, at, k, v);
     uint32_t w[VEC / 4];
-    if (at + VEC <= k) {
-      const Raw raw = *(const Raw*)(xr + at);
-#pragma unroll
-      for (int d = 0; d < VEC / 4; ++d) {
-        w[d] = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[d] |= (uint32_t)(uint8_t)(int8_t)rs(widen(raw.v[4 * d + e]))
-                  << (8 * e);
-      }
-    } else {
-#pragma unroll
-      for (int d = 0; d < VEC / 4; ++d) {
-        w[d] = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const long i = at + 4 * d + e;
-          const int v = i < k ? rs(widen(xr[i])) : 0;
-          w[d] |= (uint32_t)(uint8_t)(int8_t)v << (8 * e);
-        }
-      }
-    }
+    rs.pack(v, w);
 #pragma unroll
     for (int d = 0; d < VEC / 4; ++d) ((uint32_t*)(qr + at))[d] = w[d];
   }
@@ -203,10 +201,16 @@ __global__ __launch_bounds__(256) void quantize_long_rows_k(
 template <class T, int LANES, int CH>
 void quantize_as(const T* x, long m, long k, long stride, int8_t* q,
                  long qstride, float* scale, hipStream_t st) {
-  const long rows = 256 / LANES;
-  hipLaunchKernelGGL((quantize_rows_k<T, LANES, CH>),
-                     dim3((unsigned)((m + rows - 1) / rows)), dim3(256), 0,
-                     st, x, m, (int)k, stride, q, qstride, scale);
+  // several rows at a time once there are enough to fill the chip without
+  constexpr int ROWS = 256 / LANES, MANY = LANES <= 64 && CH == 1 ? 4 : 1;
+  const int each = m >= 4096 * ROWS ? MANY : 1;
+  const dim3 grid((unsigned)((m + ROWS * each - 1) / (ROWS * each)));
+  if (each == MANY)
+    hipLaunchKernelGGL((quantize_rows_k<T, LANES, CH, MANY>), grid, dim3(256),
+                       0, st, x, m, (int)k, stride, q, qstride, scale);
+  else
+    hipLaunchKernelGGL((quantize_rows_k<T, LANES, CH, 1>), grid, dim3(256), 0,
+                       st, x, m, (int)k, stride, q, qstride, scale);
 }
 
 template <class T>
@@ -214,19 +218,22 @@ void quantize(const T* x, long m, long k, long stride, int8_t* q,
               long qstride, float* scale, hipStream_t st) {
   // chunks of the padded row, so that its zeros are written too
   const long chunks = (qstride * (long)sizeof(T) + 15) / 16;
-  if (chunks <= 4) quantize_as<T, 4, 1>(x, m, k, stride, q, qstride, scale, st);
-  else if (chunks <= 8) quantize_as<T, 8, 1>(x, m, k, stride, q, qstride, scale, st);
-  else if (chunks <= 16) quantize_as<T, 16, 1>(x, m, k, stride, q, qstride, scale, st);
-  else if (chunks <= 32) quantize_as<T, 32, 1>(x, m, k, stride, q, qstride, scale, st);
-  else if (chunks <= 64) quantize_as<T, 64, 1>(x, m, k, stride, q, qstride, scale, st);
-  else if (chunks <= 128) quantize_as<T, 64, 2>(x, m, k, stride, q, qstride, scale, st);
-  else if (chunks <= 256) quantize_as<T, 256, 1>(x, m, k, stride, q, qstride, scale, st);
-  else if (chunks <= 512) quantize_as<T, 256, 2>(x, m, k, stride, q, qstride, scale, st);
-  else if (chunks <= 1024) quantize_as<T, 256, 4>(x, m, k, stride, q, qstride, scale, st);
-  else if (chunks <= 2048) quantize_as<T, 256, 8>(x, m, k, stride, q, qstride, scale, st);
+#define ROWS(LANES, CH) \
+  quantize_as<T, LANES, CH>(x, m, k, stride, q, qstride, scale, st)
+  if (chunks <= 4) ROWS(4, 1);
+  else if (chunks <= 8) ROWS(8, 1);
+  else if (chunks <= 16) ROWS(16, 1);
+  else if (chunks <= 32) ROWS(32, 1);
+  else if (chunks <= 64) ROWS(64, 1);
+  else if (chunks <= 128) ROWS(64, 2);
+  else if (chunks <= 256) ROWS(256, 1);
+  else if (chunks <= 512) ROWS(256, 2);
+  else if (chunks <= 1024) ROWS(256, 4);
+  else if (chunks <= 2048) ROWS(256, 8);
   else
     hipLaunchKernelGGL((quantize_long_rows_k<T>), dim3((unsigned)m),
                        dim3(256), 0, st, x, m, k, stride, q, qstride, scale);
+#undef ROWS
 }
 
 // ---------------------------------------------------------------------------
@@ -372,6 +379,97 @@ __global__ __launch_bounds__(256) void int8_few_rows_k(
   }
 }
 
+// The same for rows of x that are still floats, and few values altogether:
+// every workgroup quantises them for itself into LDS, which takes less time
+// than a launch of its own, while its first weights are on their way.
+constexpr int kFewValues = 16384;  // m * k, both rounded up (16 rows)
+
+template <class TX, class T>
+__global__ __launch_bounds__(256) void int8_linear_few_k(
+    const TX* __restrict__ x, long stride, Sources s, Scales e) {
+  constexpr int VEC = 16 / sizeof(TX);
+  __shared__ __attribute__((aligned(16))) char rows[kFewValues + 16 * 16];
+  __shared__ float part[16][4];
+  __shared__ float scale[16];
+  __shared__ v4i sums[4][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = s.rows_a, k = s.kbytes;
+  const int steps = (k + 127) / 128, tail = k - (steps - 1) * 128;
+  const int ld = steps * 128 + 16;  // rows side by side in the banks
+  const int n0 = blockIdx.x * 16, chunk = lane >> 4;
+  const char* pw = s.b[0] +
+                   (long)min(n0 + (lane & 15), s.rows_b - 1) * s.row_b;
+  // x is zero behind the row's end; there the weights are read from its
+  // beginning
+  auto weights = [&](int t, int kk) {
+    const int c = (kk * 4 + chunk) * 16;
+    return *(const v4i*)(pw + (t == steps - 1 && c >= tail
+                                   ? 0 : (long)t * 128 + c));
+  };
+  constexpr int AHEAD = 4;
+  v4i w[AHEAD][2];
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+      w[u][kk] = weights(min(wave + 4 * u, steps - 1), kk);
+  for (int r = 0; r < m; ++r) {
+    float big = 0.0f, v[VEC];
+    for (int at = threadIdx.x * VEC; at < k; at += 256 * VEC) {
+      load_chunk<TX, VEC>(x + r * stride, at, k, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) big = max_abs(big, v[i]);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) big = max_abs(big, __shfl_xor(big, d));
+    if (lane == 0) part[r][wave] = big;
+  }
+  __syncthreads();
+  for (int r = 0; r < m; ++r) {
+    float big = part[r][0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) big = max_abs(big, part[r][i]);
+    const RowScale rs(big);
+    if (threadIdx.x == 0) scale[r] = rs.scale();
+    for (int at = threadIdx.x * VEC; at < steps * 128; at += 256 * VEC) {
+      float v[VEC];
+      uint32_t q[VEC / 4];
+      load_chunk<TX, VEC>(x + r * stride, at, k, v);
+      rs.pack(v, q);
+#pragma unroll
+      for (int d = 0; d < VEC / 4; ++d)
+        ((uint32_t*)(rows + r * ld + at))[d] = q[d];
+    }
+  }
+  __syncthreads();
+  const char* px = rows + min(lane & 15, m - 1) * ld + chunk * 16;
+  v4i acc = {0, 0, 0, 0};
+  for (int t = wave; t < steps; t += 4 * AHEAD)
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int at = t + 4 * u;
+      if (at >= steps) break;
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        acc = mma(w[u][kk], *(const v4i*)(px + at * 128 + kk * 64), acc);
+        w[u][kk] = weights(min(at + 4 * AHEAD, steps - 1), kk);
+      }
+    }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int i = 1; i < 4; ++i) acc += sums[i][lane];
+    const int row = lane & 15, n = n0 + chunk * 4;
+    if (row < m && n < s.rows_b) {
+      Scales mine = e;
+      mine.xs = scale;
+      store4<T>(mine, row, n, acc);
+    }
+  }
+}
+
 template <class T>
 __global__ __launch_bounds__(256) void int8_join_k(
     const int* __restrict__ slab, int splits, long m, Scales e) {
@@ -497,4 +595,38 @@ extern "C" void launch_int8_product(const int8_t* xq, long xstride,
     product<_Float16>(s, e, p, slab, st);
   else
     product<__bf16>(s, e, p, slab, st);
+}
+
+// Whether x goes through int8_linear_few_k: few values, and weights that keep
+// the chip busy without splitting K.
+extern "C" int int8_linear_in_one(long m, long n, long k) {
+  return m <= 16 && m * ((k + 127) / 128 * 128) <= kFewValues &&
+         plan_of(m, n, k).splits == 1;
+}
+
+extern "C" void launch_int8_linear(const void* x, int xtype, long xstride,
+                                   const int8_t* wq, long wstride,
+                                   const float* ws, const float* bias, long m,
+                                   long n, long k, void* out, int dtype,
+                                   hipStream_t st) {
+  Sources s = {};
+  s.b[0] = (const char*)wq;
+  s.row_b = (unsigned)wstride;
+  s.rows_a = (int)m;
+  s.rows_b = (int)n;
+  s.kbytes = (int)k;
+  Scales e = {nullptr, ws, bias, out, n, n % 4 == 0};
+  const dim3 grid((unsigned)((n + 15) / 16));
+#define FEW(TX, T)                                                        \
+  hipLaunchKernelGGL((int8_linear_few_k<TX, T>), grid, dim3(256), 0, st, \
+                     (const TX*)x, xstride, s, e)
+#define FEW_OUT(TX)                           \
+  if (dtype == 0) FEW(TX, float);             \
+  else if (dtype == 1) FEW(TX, _Float16);     \
+  else FEW(TX, __bf16)
+  if (xtype == 0) { FEW_OUT(float); }
+  else if (xtype == 1) { FEW_OUT(_Float16); }
+  else { FEW_OUT(__bf16); }
+#undef FEW_OUT
+#undef FEW
 }

@@ -144,7 +144,7 @@ __device__ __forceinline__ void add_groups(const Panel<T, WIDE>& panel,
   }
 }
 
-// One wave's tiles into sum[tile * SIZE + row * LD + column].
+// One wave's tiles into, or onto, sum[tile * SIZE + row * LD + column].
 template <int SIZE, int LD, int COUNT>
 __device__ __forceinline__ void add_tiles(const v4d (&acc)[COUNT],
                                           double* sum, bool begin) {
@@ -167,38 +167,67 @@ __host__ __device__ constexpr int gram_shares(int nt) {
   return nt < 7 ? 1 : 2;
 }
 
-// The waves are added up in their order, and so are the workgroups
-// (gram_join_k): the same bits on every run.
+// The waves are added up in a fixed order, as many at a time as LDS has room
+// for, and so are the workgroups (gram_join_k): the same bits on every run.
 template <class T, int NT, bool WIDE>
 __global__ __launch_bounds__(gram_waves(NT) * 64) void gram_k(
     const T* __restrict__ x, long length, int n, long ld, long batch_x,
     double* __restrict__ slab) {
   constexpr int TILES = NT * (NT + 1) / 2, WAVES = gram_waves(NT);
   constexpr int SHARES = gram_shares(NT), MORE = (TILES + SHARES - 1) / SHARES;
-  __shared__ double sum[TILES * 256];
+  constexpr int ROOM = 72 / TILES, HALF = WAVES / SHARES / 2;
+  constexpr int SLOTS = ROOM < HALF ? ROOM : HALF;  // of 2 KB a tile
+  __shared__ double kept[SLOTS * TILES * 256];
   const Panel<T, WIDE> panel = {x + blockIdx.y * batch_x, length, ld, n};
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long first = (long)blockIdx.x * (WAVES / SHARES) + wave / SHARES;
+  const int lane = threadIdx.x & 63, me = wave / SHARES;
+  const long first = (long)blockIdx.x * (WAVES / SHARES) + me;
   const long stride = (long)gridDim.x * (WAVES / SHARES);
-  auto share = [&](auto from, auto count, int mine) {
+  double* out = slab + ((long)blockIdx.y * gridDim.x + blockIdx.x) *
+                           (TILES * 256);
+  auto share = [&](auto from, auto count) {
     constexpr int FROM = decltype(from)::value, COUNT = decltype(count)::value;
     v4d acc[COUNT];
 #pragma unroll
     for (int t = 0; t < COUNT; ++t) acc[t] = v4d{0, 0, 0, 0};
     add_groups<T, NT, WIDE, FROM, COUNT, true>(panel, first, stride, acc);
-    for (int w = 0; w < WAVES; ++w) {
-      if (wave == w) add_tiles<256, 16>(acc, sum + FROM * 256, w == mine);
-      __syncthreads();  // WAVES times in either share
+    // the last `take` waves give theirs to the ones before them
+    for (int left = WAVES / SHARES; left > 1;) {
+      const int take = min(SLOTS, left / 2);
+      double* slot = kept + (me - (left - take)) * (TILES * 256) + lane;
+      if (me >= left - take && me < left) {
+#pragma unroll
+        for (int t = 0; t < COUNT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            slot[((FROM + t) * 4 + i) * 64] = acc[t][i];
+      }
+      __syncthreads();
+      slot += take * (TILES * 256);
+      if (me >= left - 2 * take && me < left - take) {
+#pragma unroll
+        for (int t = 0; t < COUNT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            acc[t][i] += slot[((FROM + t) * 4 + i) * 64];
+      }
+      __syncthreads();
+      left -= take;
+    }
+    if (me == 0) {
+#pragma unroll
+      for (int t = 0; t < COUNT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          out[(FROM + t) * 256 + (4 * i + (lane >> 4)) * 16 + (lane & 15)] =
+              acc[t][i];
     }
   };
   if (wave % SHARES == 0)
-    share(Count<0>(), Count<MORE>(), 0);
+    share(Count<0>(), Count<MORE>());
   else
     share(Count<(SHARES > 1 ? MORE : 0)>(),
-          Count<(SHARES > 1 ? TILES - MORE : 1)>(), 1);
-  double* out = slab + ((long)blockIdx.y * gridDim.x + blockIdx.x) *
-                           (TILES * 256);
-  for (int i = threadIdx.x; i < TILES * 256; i += WAVES * 64) out[i] = sum[i];
+          Count<(SHARES > 1 ? TILES - MORE : 1)>());
 }
 
 __global__ __launch_bounds__(1024) void gram_join_k(
@@ -453,7 +482,7 @@ __device__ __forceinline__ void apply_rows(const double* qs,
 }
 
 template <class T, int NT, bool WIDE>
-__global__ __launch_bounds__(256, NT <= 4 ? 3 : 1) void apply_k(
+__global__ __launch_bounds__(256, NT > 4 ? 1 : WIDE ? 3 : 4) void apply_k(
     const T* __restrict__ x, long length, int n, long ld, long batch_x,
     const double* __restrict__ factor, T* __restrict__ out, long ld_out,
     long batch_out) {
@@ -904,7 +933,7 @@ extern "C" void launch_apply(const void* x, int dtype, int wide, long length,
                              long batch_out, hipStream_t st) {
   const long groups = (length + 15) / 16;
   const long want = (groups + 15) / 16;
-  const long most = n <= 64 ? 768 : 256;  // what a CU has room for
+  const long most = n > 64 ? 256 : wide ? 768 : 1024;  // what fits at once
   const int blocks = (int)(want < 1 ? 1 : want > most ? most : want);
 #define CALL(T)                                                           \
   apply_type((const T*)x, wide, length, n, ld, batch_x, batch, factor,    \

@@ -65,32 +65,36 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return q.to(torch.int8), scale
 
 
-def _check_product(xq, x_scale, wq, w_scale, bias, out_dtype) -> None:
-    for name, q in (("xq", xq), ("wq", wq)):
-        if q.dim() != 2:
-            raise ValueError(f"{name} must be 2-D, got {q.dim()}-D")
-        if q.dtype != torch.int8:
-            raise TypeError(f"{name} must be int8, got {q.dtype}")
-    if xq.shape[1] != wq.shape[1]:
-        raise ValueError(f"xq has rows of {xq.shape[1]} values and wq of "
-                         f"{wq.shape[1]}")
-    if xq.shape[1] > MAX_K:
+def _check_int8(q: torch.Tensor, name: str) -> None:
+    if q.dim() != 2:
+        raise ValueError(f"{name} must be 2-D, got {q.dim()}-D")
+    if q.dtype != torch.int8:
+        raise TypeError(f"{name} must be int8, got {q.dtype}")
+
+
+def _check_vector(s: torch.Tensor, size: int, device, name: str) -> None:
+    if s.dim() != 1 or s.shape[0] != size:
+        raise ValueError(f"{name} must have shape ({size},), got "
+                         f"{tuple(s.shape)}")
+    if s.dtype != torch.float32:
+        raise TypeError(f"{name} must be float32, got {s.dtype}")
+    if s.device != device:
+        raise ValueError(f"{name} is on {s.device}, the rows are on {device}")
+
+
+def _check_weights(x, x_name, wq, w_scale, bias, out_dtype) -> None:
+    _check_int8(wq, "wq")
+    if x.shape[1] != wq.shape[1]:
+        raise ValueError(f"{x_name} has rows of {x.shape[1]} values and wq "
+                         f"of {wq.shape[1]}")
+    if x.shape[1] > MAX_K:
         raise ValueError(f"rows of more than {MAX_K} values could overflow "
-                         f"the 32-bit sums, got {xq.shape[1]}")
-    for name, s, size in (("x_scale", x_scale, xq.shape[0]),
-                          ("w_scale", w_scale, wq.shape[0]),
-                          ("bias", bias, wq.shape[0])):
-        if s is None and name == "bias":
-            continue
-        if s.shape != (size,):
-            raise ValueError(f"{name} must have shape ({size},), got "
-                             f"{tuple(s.shape)}")
-        if s.dtype != torch.float32:
-            raise TypeError(f"{name} must be float32, got {s.dtype}")
-    for name, t in (("x_scale", x_scale), ("wq", wq), ("w_scale", w_scale),
-                    ("bias", bias)):
-        if t is not None and t.device != xq.device:
-            raise ValueError(f"{name} is on {t.device}, xq on {xq.device}")
+                         f"the 32-bit sums, got {x.shape[1]}")
+    if wq.device != x.device:
+        raise ValueError(f"wq is on {wq.device}, the rows are on {x.device}")
+    _check_vector(w_scale, wq.shape[0], x.device, "w_scale")
+    if bias is not None:
+        _check_vector(bias, wq.shape[0], x.device, "bias")
     if out_dtype not in _FLOATS:
         raise TypeError(f"out_dtype must be float32, float16 or bfloat16, "
                         f"got {out_dtype}")
@@ -106,7 +110,9 @@ def int8_matmul(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor,
     once. Rows that do not begin at multiples of 16 bytes (``quantize_rows``
     lays them out so) are copied first.
     """
-    _check_product(xq, x_scale, wq, w_scale, bias, out_dtype)
+    _check_int8(xq, "xq")
+    _check_weights(xq, "xq", wq, w_scale, bias, out_dtype)
+    _check_vector(x_scale, xq.shape[0], xq.device, "x_scale")
     if use_hip(xq):
         return hip_ext().int8_product(xq, x_scale, wq, w_scale, bias,
                                       out_dtype)
@@ -128,5 +134,8 @@ def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
     """
     _check_floats(x, "x")
     out_dtype = x.dtype if out_dtype is None else out_dtype
+    _check_weights(x, "x", wq, w_scale, bias, out_dtype)
+    if use_hip(x):
+        return hip_ext().int8_linear(x, wq, w_scale, bias, out_dtype)
     xq, x_scale = quantize_rows(x)
     return int8_matmul(xq, x_scale, wq, w_scale, bias, out_dtype)

@@ -170,6 +170,22 @@ def test_linear_is_quantize_then_product():
                                             torch.bfloat16))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_gpu_linear_is_quantize_then_product(dtype):
+    # to the bit, in one launch or two, for values on the halves too
+    for x in (_halves(dtype), _rows(5, 900, dtype), _rows(40, 900, dtype),
+              _rows(16, 1600, dtype)[:, ::2], _rows(9, 100, dtype)[:, 1:]):
+        x = x.cuda()
+        wq, ws = ops.quantize_rows(_rows(600, x.shape[1]).cuda())
+        b = torch.randn(600, device="cuda")
+        xq, xs = ops.quantize_rows(x)
+        assert torch.equal(ops.int8_linear(x, wq, ws, b),
+                           ops.int8_matmul(xq, xs, wq, ws, b, dtype))
+        assert torch.equal(ops.int8_linear(x, wq, ws),
+                           ops.int8_matmul(xq, xs, wq, ws, None, dtype))
+
+
 def test_bad_rows_give_nan_alone():
     x, w = _rows(5, 30), _rows(4, 30)
     x[1, 2], x[3, 0] = float("inf"), float("nan")
@@ -204,6 +220,12 @@ def test_refusals():
         ops.int8_matmul(long, s[:1], long, s[:1])
     with pytest.raises(TypeError, match="float32"):
         ops.int8_linear(torch.ones(3, 3, dtype=torch.int32), q, s)
+    with pytest.raises(ValueError, match="rows of"):
+        ops.int8_linear(x[:, :3], q, s)
+    with pytest.raises(ValueError, match="w_scale"):
+        ops.int8_linear(x, q, s[:1])
+    with pytest.raises(TypeError, match="int8"):
+        ops.int8_linear(x, x, s)
 
 
 def _check_estimators():
@@ -413,10 +435,13 @@ def test_gpu_product_largest_sums_are_exact():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [1, 20, 100])
-def test_gpu_linear(m):
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 127), (1, 128), (1, 8192),
+                                 (1, 16384), (1, 16385), (2, 5001), (3, 500),
+                                 (7, 2300), (16, 1000), (16, 1025), (17, 90),
+                                 (20, 500), (100, 500)])
+def test_gpu_linear(m, k):
     for dtype in FLOATS:
-        x, w = _rows(m, 500, dtype), _rows(77, 500)
+        x, w = _rows(m, k, dtype), _rows(77, k)
         wq, ws = ops.quantize_rows(w)
         b = torch.randn(77)
         want = ops.int8_linear(x, wq, ws, b, torch.float32)
