@@ -76,7 +76,8 @@ torch::TensorOptions doubles(const torch::Tensor& t) {
   return t.options().dtype(torch::kFloat64);
 }
 
-// The upper 16 x 16 tiles of X X^T of the shorter side, [batch, tiles * 256].
+// The upper 16 x 16 tiles of X X^T of the shorter side, [batch, tiles * 256],
+// its rows and columns in the kernels' order.
 torch::Tensor gram_of(const Matrices& v) {
   const long nt = (v.n + 15) / 16, size = nt * (nt + 1) / 2 * 256;
   const int parts = gram_parts(v.length, v.n, (int)v.batch);

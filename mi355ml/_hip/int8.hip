@@ -94,14 +94,38 @@ template <class T, int VEC> struct Chunk {
   struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[VEC]; };
 };
 
-// VEC values from the row's at-th on, zeros behind its end.
+// VEC values from the row's at-th on, zeros behind its end. Rows of VEC
+// values and more are read without a branch (the compiler waits for the loads
+// before one): the last VEC values in place of a piece that the end cuts, and
+// then moved to its beginning.
+template <class T, int VEC>
+__device__ __forceinline__ typename Chunk<T, VEC>::Raw load_raw(const T* row,
+                                                                long at,
+                                                                long k) {
+  return *(const typename Chunk<T, VEC>::Raw*)(row + min(at, k - VEC));
+}
+template <class T, int VEC>
+__device__ __forceinline__ void place_raw(
+    const typename Chunk<T, VEC>::Raw& raw, long at, long k, float (&v)[VEC]) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) v[e] = widen(raw.v[e]);
+  const long off = at + VEC - k;  // values that are not there
+  if (off <= 0) return;
+#pragma unroll
+  for (int d = VEC / 2; d > 0; d >>= 1)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (off & d) v[e] = e + d < VEC ? v[e + d] : 0.0f;
+  if (off >= VEC) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
+  }
+}
 template <class T, int VEC>
 __device__ __forceinline__ void load_chunk(const T* row, long at, long k,
                                            float (&v)[VEC]) {
-  if (at + VEC <= k) {
-    const auto raw = *(const typename Chunk<T, VEC>::Raw*)(row + at);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = widen(raw.v[e]);
+  if (k >= VEC) {
+    place_raw<T, VEC>(load_raw<T, VEC>(row, at, k), at, k, v);
   } else {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = at + e < k ? widen(row[at + e]) : 0.0f;
@@ -122,13 +146,26 @@ __global__ __launch_bounds__(256) void quantize_rows_k(
   const int lane = threadIdx.x % LANES;
   const long first = (long)blockIdx.x * (ROWS * EACH) + threadIdx.x / LANES;
   float v[EACH][CH][VEC];
+  if (k >= VEC) {
+    typename Chunk<T, VEC>::Raw raw[EACH][CH];
 #pragma unroll
-  for (int r = 0; r < EACH; ++r) {
-    const long row = min(first + r * ROWS, m - 1);
+    for (int r = 0; r < EACH; ++r)
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-      load_chunk<T, VEC>(x + row * stride, (c * LANES + lane) * VEC, k,
-                         v[r][c]);
+      for (int c = 0; c < CH; ++c)
+        raw[r][c] = load_raw<T, VEC>(x + min(first + r * ROWS, m - 1) * stride,
+                                     (c * LANES + lane) * VEC, k);
+#pragma unroll
+    for (int r = 0; r < EACH; ++r)
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        place_raw<T, VEC>(raw[r][c], (c * LANES + lane) * VEC, k, v[r][c]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < EACH; ++r)
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        load_chunk<T, VEC>(x + min(first + r * ROWS, m - 1) * stride,
+                           (c * LANES + lane) * VEC, k, v[r][c]);
   }
 #pragma unroll
   for (int r = 0; r < EACH; ++r) {
@@ -510,7 +547,7 @@ Plan plan_of(long m, long n, long k) {
         const int per = (steps + splits - 1) / splits;
         const double join =
             splits > 1 ? 4.0 + 8e-6 * splits * m * n / 4.0 : 0.0;
-        const double t = per * step_time(c, tm * tn * splits) + join;
+        const double t = tile_time(c, tm * tn * splits, per) + join;
         if (t < best) {
           best = t;
           p.size = c.size;
@@ -539,8 +576,7 @@ void product(const Sources& s, const Scales& e, const Plan& p, int* slab,
   else if (p.rows == 32) FEW(2);
   else if (p.rows == 64) FEW(4);
   else {
-    const bool alone = (long)p.tm * p.tn * p.splits <= 256;
-    BY_TILE_SIZE(p.size, alone, TILE)
+    BY_TILE_SIZE(p.size, (long)p.tm * p.tn * p.splits, TILE)
   }
 #undef FEW
 #undef TILE

@@ -49,33 +49,51 @@ __host__ __device__ constexpr int upper(int nt, int i, int j) {
   return i * nt - i * (i - 1) / 2 + (j - i);
 }
 
-template <class T> struct Four {
-  struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[4]; };
+template <class T, int N> struct Some {
+  struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[N]; };
 };
 
-// Four values side by side, zeros from the n-th on.
-template <class T>
-__device__ __forceinline__ void load4(const T* p, long n, float (&v)[4]) {
-  if (n >= 4) {
-    const auto raw = *(const typename Four<T>::Raw*)p;
+// N values side by side, zeros from the left-th on.
+template <class T, int N>
+__device__ __forceinline__ void load_side(const T* p, long left,
+                                          float (&v)[N]) {
+  if (left >= N) {
+    const auto raw = *(const typename Some<T, N>::Raw*)p;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = (float)raw.v[u];
+    for (int u = 0; u < N; ++u) v[u] = (float)raw.v[u];
   } else {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = u < n ? (float)p[u] : 0.0f;
+    for (int u = 0; u < N; ++u) v[u] = u < left ? (float)p[u] : 0.0f;
   }
 }
 
-// Element (p, q) of a panel stands at p * sp + q * sq: p counts the longer
-// side, q the shorter one. WIDE: sp is 1, otherwise sq is.
+// Element (p, q) of a panel stands at p * ld + q, or for WIDE at q * ld + p:
+// p counts the longer side, q the n columns of the shorter one.
 template <class T, bool WIDE>
 struct Panel {
   const T* x;
   long length, ld;
   int n;
   __device__ __forceinline__ float at(long p, int q) const {
-    return p < length && q < n ? (float)x[WIDE ? q * ld + p : p * ld + q]
-                               : 0.0f;
+    return (float)x[WIDE ? q * ld + p : p * ld + q];
+  }
+};
+
+// Which columns stand in place c of the NT tiles: c NT + i in tile i, so that
+// a lane has NT of them side by side. The place behind the last full one
+// takes the last NT columns, and those of them that are new count. So every
+// load of NT values stays in its row, and none needs a branch of its own:
+// with branches around them the compiler waits for loads too early.
+template <int NT>
+struct Columns {
+  int n, full, rest;
+  __device__ __forceinline__ explicit Columns(int n)
+      : n(n), full(n / NT), rest(n % NT) {}
+  __device__ __forceinline__ int first(int c) const {
+    return c < full ? c * NT : c == full && rest ? n - NT : 0;
+  }
+  __device__ __forceinline__ bool counts(int c, int i) const {
+    return c < full || (c == full && i >= NT - rest);
   }
 };
 
@@ -84,62 +102,99 @@ struct Panel {
 // A wave takes 16 positions of the longer side at a time and has all tiles in
 // registers, the next 16 positions on their way.
 // ---------------------------------------------------------------------------
+// ---------------------------------------------------------------------------
 template <class T, int NT, bool WIDE>
-__device__ __forceinline__ void load_group(const Panel<T, WIDE>& panel, long g,
+__device__ __forceinline__ void load_group(const Panel<T, WIDE>& panel,
+                                           const Columns<NT>& columns, long g,
                                            float (&v)[4][NT]) {
   const int c = threadIdx.x & 15, h = (threadIdx.x & 63) >> 4;
+  const int q0 = columns.first(c);
+  if (WIDE) {
+    // the sum over the longer side may take it in any order: four positions
+    // side by side for a lane, the last four at its end
+    const long p = min(g * 16 + h * 4, panel.length - 4);
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int q = i * 16 + c;
-    if (WIDE) {
-      // the sum over the longer side may take it in any order: four
-      // positions side by side for a lane
-      const long p = g * 16 + h * 4;
-      float e[4] = {0, 0, 0, 0};
-      if (q < panel.n) load4(panel.x + q * panel.ld + p, panel.length - p, e);
+    for (int i = 0; i < NT; ++i) {
+      const auto raw = *(const typename Some<T, 4>::Raw*)(
+          panel.x + (q0 + i) * panel.ld + p);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) v[t][i] = e[t];
-    } else {
+      for (int t = 0; t < 4; ++t) v[t][i] = (float)raw.v[t];
+    }
+  } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) v[t][i] = panel.at(g * 16 + t * 4 + h, q);
+    for (int t = 0; t < 4; ++t) {
+      const long p = min(g * 16 + t * 4 + h, panel.length - 1);
+      const auto raw =
+          *(const typename Some<T, NT>::Raw*)(panel.x + p * panel.ld + q0);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) v[t][i] = (float)raw.v[i];
     }
   }
 }
 
-// Tiles FROM to FROM + COUNT of groups first, first + stride, ... added to
-// acc; AHEAD: with the next group on its way.
+// Tiles FROM to FROM + COUNT of group g, whose values are v, added to acc.
+template <int NT, bool WIDE, int FROM, int COUNT>
+__device__ __forceinline__ void add_group(const Columns<NT>& columns,
+                                          long length, long g,
+                                          const float (&v)[4][NT],
+                                          v4d (&acc)[COUNT]) {
+  const int c = threadIdx.x & 15, h = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    // wide: positions that an earlier lane has too do not count twice
+    const long p = g * 16 + (WIDE ? h * 4 : t * 4 + h);
+    const bool here =
+        WIDE ? p < length && min(p, length - 4) + t >= p : p < length;
+    double w[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+      w[i] = here && columns.counts(c, i) ? (double)v[t][i] : 0.0;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = i; j < NT; ++j) {
+        const int k = upper(NT, i, j);
+        if (k >= FROM && k < FROM + COUNT)
+          acc[k - FROM] = mma64(w[i], w[j], acc[k - FROM]);
+      }
+  }
+}
+
+// Groups first, first + stride, ...; AHEAD: with the next on its way.
 template <class T, int NT, bool WIDE, int FROM, int COUNT, bool AHEAD>
 __device__ __forceinline__ void add_groups(const Panel<T, WIDE>& panel,
                                            long first, long stride,
                                            v4d (&acc)[COUNT]) {
+  const Columns<NT> columns(panel.n);
   const long groups = (panel.length + 15) / 16;
-  float now[4][NT], next[4][NT];
-  long g = first;
-  if (g < groups) load_group(panel, g, now);
-  for (; g < groups; g += stride) {
-    if (AHEAD && g + stride < groups) load_group(panel, g + stride, next);
+  if (first >= groups) return;
+  float now[4][NT];
+  if (WIDE && panel.length < 4) {  // one tile, and no four side by side
+    const int c = threadIdx.x & 15, h = (threadIdx.x & 63) >> 4;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      double v[NT];
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int i = 0; i < NT; ++i) v[i] = (double)now[t][i];
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = i; j < NT; ++j) {
-          constexpr int LAST = FROM + COUNT;
-          const int k = upper(NT, i, j);
-          if (k >= FROM && k < LAST)
-            acc[k - FROM] = mma64(v[i], v[j], acc[k - FROM]);
-        }
-    }
+      for (int i = 0; i < NT; ++i) {
+        const bool here = h == 0 && t < panel.length && columns.counts(c, i);
+        now[t][i] = here ? panel.at(t, columns.first(c) + i) : 0.0f;
+      }
+    // as if they were four
+    add_group<NT, WIDE, FROM, COUNT>(columns, 4, 0, now, acc);
+    return;
+  }
+  load_group(panel, columns, first, now);
+  for (long g = first; g < groups; g += stride) {
     if (AHEAD) {
+      float next[4][NT];
+      load_group(panel, columns, min(g + stride, groups - 1), next);
+      add_group<NT, WIDE, FROM, COUNT>(columns, panel.length, g, now, acc);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < NT; ++i) now[t][i] = next[t][i];
-    } else if (g + stride < groups) {
-      load_group(panel, g + stride, now);
+    } else {
+      add_group<NT, WIDE, FROM, COUNT>(columns, panel.length, g, now, acc);
+      if (g + stride < groups) load_group(panel, columns, g + stride, now);
     }
   }
 }
@@ -271,7 +326,7 @@ struct Factor {
   static constexpr int kLds = 2 * kMatrix > N * N ? 2 * kMatrix : N * N;
 
   // G_0 in s (kMatrix values) -> this wave's tiles of Q, and where they are
-  static __device__ __forceinline__ void run(double* s, int n, int steps,
+  static __device__ __forceinline__ void run(double* s, int steps,
                                              double a, double b, double c,
                                              int (&ti)[MINE], int (&tj)[MINE],
                                              v4d (&q)[MINE]) {
@@ -279,7 +334,7 @@ struct Factor {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, h = lane >> 4;
     double trace = 0.0;
-    for (int k = lane; k < n; k += 64)
+    for (int k = lane; k < N; k += 64)  // zeros where there is no column
       trace += s0[upper(NT, k >> 4, k >> 4) * SIZE + (k & 15) * (LD + 1)];
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) trace += __shfl_xor(trace, d);
@@ -379,18 +434,27 @@ struct Factor {
     return (int)(threadIdx.x >> 6) + t * kFactorWaves < TILES;
   }
 
-  // Q in the order in which the matrix instruction takes it as k x column:
-  // the k of an instruction are 16 s + 4 (lane / 16) + t, so that a lane's
-  // four of them stand side by side in a tall panel.
-  static __device__ __forceinline__ int place(int k, int column) {
-    const int s = k >> 4, h = (k >> 2) & 3, t = k & 3;
-    return ((s * 4 + t) * NT + (column >> 4)) * 64 + h * 16 + (column & 15);
-  }
-
-  static __device__ __forceinline__ void store(const int (&ti)[MINE],
+  // Q into `out`, in LDS, in the order in which the matrix instruction takes
+  // it: columns of the panel (k) by rows of Q (z). A lane takes the k of an
+  // instruction from four columns side by side: 16 s + 4 (lane / 16) + t, and
+  // behind the last full four the last four columns again, where what is not
+  // new meets zeros.
+  static __device__ __forceinline__ void store(int n, const int (&ti)[MINE],
                                                const int (&tj)[MINE],
                                                const v4d (&q)[MINE],
                                                double* out) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < N * N; i += kFactorWaves * 64) out[i] = 0.0;
+    __syncthreads();
+    const Columns<NT> columns(n);
+    auto put = [&](int y, int z, double v) {
+      const int c = y & 15, i = y >> 4;
+      if (!columns.counts(c, i)) return;
+      int k = columns.first(c) + i;
+      if (n >= 4 && k >= n / 4 * 4) k = n / 4 * 4 + k - (n - 4);
+      const int s = k >> 4, h = (k >> 2) & 3, t = k & 3;
+      out[((s * 4 + t) * NT + (z >> 4)) * 64 + h * 16 + (z & 15)] = v;
+    };
     const int col = threadIdx.x & 15, h = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int t = 0; t < MINE; ++t)
@@ -398,9 +462,10 @@ struct Factor {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int y = ti[t] * 16 + 4 * i + h, z = tj[t] * 16 + col;
-          out[place(y, z)] = q[t][i];
-          out[place(z, y)] = q[t][i];
+          put(y, z, q[t][i]);
+          if (ti[t] != tj[t]) put(z, y, q[t][i]);
         }
+    __syncthreads();
   }
 };
 
@@ -409,34 +474,42 @@ __global__ __launch_bounds__(kFactorWaves * 64) void factor_k(
     const double* __restrict__ gram, int n, int steps, double a, double b,
     double c, double* __restrict__ out) {
   typedef Factor<NT> F;
-  __shared__ double s[2 * F::kMatrix];
+  __shared__ double s[F::kLds];
   gram += (long)blockIdx.x * F::TILES * 256;
   for (int i = threadIdx.x; i < F::TILES * 256; i += kFactorWaves * 64)
     s[(i >> 8) * F::SIZE + ((i >> 4) & 15) * F::LD + (i & 15)] = gram[i];
   __syncthreads();
   int ti[F::MINE], tj[F::MINE];
   v4d q[F::MINE];
-  F::run(s, n, steps, a, b, c, ti, tj, q);
-  F::store(ti, tj, q, out + (long)blockIdx.x * F::N * F::N);
+  F::run(s, steps, a, b, c, ti, tj, q);
+  F::store(n, ti, tj, q, s);
+  out += (long)blockIdx.x * F::N * F::N;
+  for (int i = threadIdx.x; i < F::N * F::N; i += kFactorWaves * 64)
+    out[i] = s[i];
 }
 
 // ---------------------------------------------------------------------------
-// Out = Q X for 16 positions of the longer side, Q in LDS as Factor::place
-// says.
+// Out = Q X for 16 positions of the longer side, Q in LDS as Factor::store
+// leaves it. What is loaded in place of columns that are not there meets
+// zeros (an infinity or NaN among it has made all of Q NaN).
 // ---------------------------------------------------------------------------
 template <class T, int NT, bool WIDE>
 __device__ __forceinline__ void load_rows(const Panel<T, WIDE>& panel, long g,
                                           float (&v)[NT][4]) {
   const int c = threadIdx.x & 15, h = (threadIdx.x & 63) >> 4;
-  const long p = g * 16 + c;
+  const long p = min(g * 16 + c, panel.length - 1);
+  const int n = panel.n;
 #pragma unroll
   for (int s = 0; s < NT; ++s) {
-    const int q = s * 16 + h * 4;
-    if (!WIDE && p < panel.length) {
-      load4(panel.x + p * panel.ld + q, panel.n - q, v[s]);
-    } else {
+    const int q = min(s * 16 + h * 4, max(n - 4, 0));
+    if (WIDE || n < 4) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) v[s][t] = panel.at(p, q + t);
+      for (int t = 0; t < 4; ++t) v[s][t] = panel.at(p, min(q + t, n - 1));
+    } else {
+      const auto raw =
+          *(const typename Some<T, 4>::Raw*)(panel.x + p * panel.ld + q);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) v[s][t] = (float)raw.v[t];
     }
   }
 }
@@ -461,24 +534,38 @@ __device__ __forceinline__ void apply_rows(const double* qs,
         acc[j] = WIDE ? mma64(f, w, acc[j]) : mma64(w, f, acc[j]);
       }
       // or the compiler reads all of Q ahead, into registers that are not
-      // there
+      // there (60 columns of a million rows: 150 us, without it 310)
       if (t == 3) __builtin_amdgcn_sched_barrier(0);
     }
+  const Columns<NT> columns(panel.n);
+  if (WIDE) {
+    const long p = g * 16 + c;
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int place = 4 * i + h;
+        if (columns.counts(place, j) && p < panel.length)
+          out[(columns.first(place) + j) * ld_out + p] = (T)(float)acc[j][i];
+      }
+  } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const T y = (T)(float)acc[j][i];
-      if (WIDE) {
-        const long p = g * 16 + c;
-        const int q = j * 16 + 4 * i + h;
-        if (q < panel.n && p < panel.length) out[q * ld_out + p] = y;
+      const long p = g * 16 + 4 * i + h;
+      if (p >= panel.length) continue;
+      typename Some<T, NT>::Raw y;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) y.v[j] = (T)(float)acc[j][i];
+      T* to = out + p * ld_out + columns.first(c);
+      if (c < columns.full) {
+        *(typename Some<T, NT>::Raw*)to = y;
       } else {
-        const long p = g * 16 + 4 * i + h;
-        const int q = j * 16 + c;
-        if (q < panel.n && p < panel.length) out[p * ld_out + q] = y;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          if (columns.counts(c, j)) to[j] = y.v[j];
       }
     }
+  }
 }
 
 template <class T, int NT, bool WIDE>
@@ -499,7 +586,7 @@ __global__ __launch_bounds__(256, NT > 4 ? 1 : WIDE ? 3 : 4) void apply_k(
   for (int i = threadIdx.x; i < N * N; i += 256) qs[i] = factor[i];
   __syncthreads();
   for (; g < groups; g += stride) {
-    if (g + stride < groups) load_rows(panel, g + stride, next);
+    load_rows(panel, min(g + stride, groups - 1), next);
     apply_rows<T, NT, WIDE>(qs, panel, g, now, out, ld_out);
 #pragma unroll
     for (int s = 0; s < NT; ++s)
@@ -535,10 +622,8 @@ __global__ __launch_bounds__(kFactorWaves * 64) void small_k(
   }
   int ti[F::MINE], tj[F::MINE];
   v4d q[F::MINE];
-  F::run(s, n, steps, a, b, c, ti, tj, q);
-  __syncthreads();
-  F::store(ti, tj, q, s);
-  __syncthreads();
+  F::run(s, steps, a, b, c, ti, tj, q);
+  F::store(n, ti, tj, q, s);
   float v[NT][4];
   for (long g = wave; g < (length + 15) / 16; g += kFactorWaves) {
     load_rows(panel, g, v);
@@ -563,7 +648,7 @@ __global__ __launch_bounds__(256) void squares_k(
     const T* row = x + r * ld;
     for (int k = threadIdx.x * 4; k < cols; k += 1024) {
       float e[4];
-      load4(row + k, cols - k, e);
+      load_side(row + k, cols - k, e);
 #pragma unroll
       for (int u = 0; u < 4; ++u) v += (double)e[u] * (double)e[u];
     }
@@ -630,7 +715,7 @@ __global__ __launch_bounds__(256) void split_k(
   for (int i = threadIdx.x; i < 64 * 16; i += 256) {
     const int r = i >> 4, k = (i & 15) * 4;
     float y[4] = {0, 0, 0, 0};
-    if (r0 + r < rows) load4(x + (r0 + r) * ld + c0 + k, cols - c0 - k, y);
+    if (r0 + r < rows) load_side(x + (r0 + r) * ld + c0 + k, cols - c0 - k, y);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       tile[r][k + u] = fine ? ldexpf(y[u], 14 - e) : 0.0f;
@@ -782,7 +867,8 @@ void step_as(Sources s, Step p, int batch, hipStream_t st) {
   int size = 0;
   double best = 0;
   for (const TileCost& c : kTiles) {
-    const double t = step_time(c, tiles_of(c.size) * batch);
+    const double t = tile_time(c, tiles_of(c.size) * batch,
+                               (long)s.parts * s.kbytes / kStep);
     if (!size || t < best) {
       size = c.size;
       best = t;
@@ -790,12 +876,11 @@ void step_as(Sources s, Step p, int batch, hipStream_t st) {
   }
   p.tm = (s.rows_a + size - 1) / size;
   p.tn = (s.rows_b + size - 1) / size;
-  const bool alone = tiles_of(size) * batch <= 256;
   const dim3 grid((unsigned)tiles_of(size), batch);
 #define STEP(BM, WM, WN, STAGES, GROUPS)                              \
   hipLaunchKernelGGL((step_k<OUT, BM, WM, WN, STAGES, GROUPS>), grid, \
                      dim3(GROUPS * (BM / WM) * (BM / WN) * 64), 0, st, s, p)
-  BY_TILE_SIZE(size, alone, STEP)
+  BY_TILE_SIZE(size, tiles_of(size) * batch, STEP)
 #undef STEP
 }
 

@@ -327,30 +327,35 @@ struct Tile {
   }
 };
 
-// Sizes of square tiles, and what a step takes (us, fp16 and int8 alike, from
-// products of 256^2 to 4096^2 outputs): as long as a CU has one tile at most,
-// and for each further tile that a CU gets. Large tiles read less for what
-// they compute, small ones leave less of the chip idle.
+// Sizes of square tiles, and what they take in us, from products of 256^2 to
+// 4096^2 outputs, fp16 and int8 alike: a step as long as a CU has one tile at
+// most, a step for each further tile that a CU gets, and what stands before
+// the first step and behind the last (from 100,000 x 1000 outputs of one
+// step, where nothing else counts). Large tiles read less for what they
+// compute, small ones leave less of the chip idle, and as several of them
+// share a CU one's end goes along with another's steps.
 struct TileCost {
   int size;
-  double first, more;
+  double first, more, ends;
 };
-constexpr TileCost kTiles[] = {{256, 1.75, 1.75}, {192, 1.0, 1.1},
-                               {128, 0.6, 0.57},  {96, 0.41, 0.37},
-                               {64, 0.28, 0.21},  {32, 0.2, 0.1}};
+constexpr TileCost kTiles[] = {
+    {256, 1.75, 1.75, 20.0}, {192, 1.0, 1.1, 11.0}, {128, 0.6, 0.57, 4.5},
+    {96, 0.41, 0.37, 2.8},   {64, 0.28, 0.21, 1.3}, {32, 0.2, 0.1, 0.5}};
 
-// us for one step of `tiles` tiles
-inline double step_time(const TileCost& c, long tiles) {
+// us for `tiles` tiles of `steps` steps
+inline double tile_time(const TileCost& c, long tiles, long steps) {
   const double rounds = (double)((tiles + 255) / 256);
-  return rounds <= 1 ? c.first : c.more * rounds > c.first ? c.more * rounds
-                                                            : c.first;
+  const double step =
+      rounds <= 1 || c.more * rounds < c.first ? c.first : c.more * rounds;
+  return step * steps + c.ends * rounds;
 }
 
 // LAUNCH(BM, WM, WN, STAGES, GROUPS) for tiles of `size`. Up to 128, where a
-// CU gets one tile at most (`alone`), four steps in LDS are quicker (2048^2
-// outputs by 128: 39 us for 64 steps, with two 47), otherwise two, so that
-// several workgroups fit (4096^2 by 128: 144 us, with four 159).
-#define BY_TILE_SIZE(size, alone, LAUNCH)          \
+// CU gets one tile at most, four steps in LDS are quicker (2048^2 outputs by
+// 128: 39 us for 64 steps, with two 47), otherwise two, so that several
+// workgroups fit (4096^2 by 128: 144 us, with four 159).
+#define BY_TILE_SIZE(size, tiles, LAUNCH)          \
+  const bool alone = (tiles) <= 256;               \
   switch (size) {                                  \
     case 256: LAUNCH(256, 128, 64, 2, 1); break;   \
     case 192: LAUNCH(192, 96, 48, 3, 1); break;    \

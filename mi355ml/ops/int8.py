@@ -43,8 +43,9 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     that holds an infinity or NaN has scale NaN and zeros for q, so that it
     gives NaN wherever it is used.
 
-    The rows of q begin at multiples of 16 bytes, as the product wants them:
-    q is a view of a wider matrix where k is no such multiple.
+    The rows of q begin at multiples of 16 bytes (of 128 from k = 1024 on),
+    as the product wants them: q is a view of a wider matrix where k is no
+    such multiple.
     """
     _check_floats(x, "x")
     if use_hip(x):
