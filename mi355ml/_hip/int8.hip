@@ -293,15 +293,13 @@ template <class T> __device__ __forceinline__ T narrow(float v) {
 // Four columns side by side of one row: y = acc xs ws + bias, rounded once.
 template <class T>
 __device__ __forceinline__ void store4(const Scales& e, long m, long n,
-                                       const v4i& acc) {
-  const float xs = e.xs[m];
+                                       const v4i& acc, float xs, const v4f& ws,
+                                       const v4f& bias) {
   T* out = (T*)e.out + m * e.n + n;
   T v[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    if (n + r < e.n)
-      v[r] = narrow<T>(fmaf((float)acc[r] * xs, e.ws[n + r],
-                            e.bias ? e.bias[n + r] : 0.0f));
+    v[r] = narrow<T>(fmaf((float)acc[r] * xs, ws[r], bias[r]));
   if (e.vec && n + 4 <= e.n) {
     struct __attribute__((aligned(4 * sizeof(T)))) Four { T v[4]; };
     *(Four*)out = Four{v[0], v[1], v[2], v[3]};
@@ -312,32 +310,61 @@ __device__ __forceinline__ void store4(const Scales& e, long m, long n,
   }
 }
 
-// `slab` not null: the sums of this split of K, for joining later.
+// The scales and bias of four columns, whatever they are behind the last.
+__device__ __forceinline__ void four_columns(const Scales& e, long n, v4f& ws,
+                                             v4f& bias) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const long at = min(n + r, e.n - 1);
+    ws[r] = e.ws[at];
+    bias[r] = e.bias ? e.bias[at] : 0.0f;
+  }
+}
+
+// `slab` not null: the sums of this split of K, for joining later. The splits
+// take K's steps in turn, so that those that run at the same time read side by
+// side in every row (4096 rows of 50000, 4 splits).
 template <class T, int BM, int WM, int WN, int STAGES, int GROUPS>
 __global__ __launch_bounds__(GROUPS * (BM / WM) * (BM / WN) * 64)
 void int8_tile_k(
-    Sources s, Scales e, int tm, int tn, int per, int* __restrict__ slab) {
+    Sources s, Scales e, int tm, int tn, int* __restrict__ slab) {
   constexpr int BN = BM;
-  typedef Tile<v4i, BM, BN, WM, WN, STAGES, GROUPS> P;
+  typedef Tile<v4i, BM, BN, WM, WN, STAGES, GROUPS, 1> P;
   __shared__ __attribute__((aligned(16))) char lds[P::kLds];
   int ti, tj;
   banded(xcd_contiguous(blockIdx.x, gridDim.x), tm, tn, ti, tj);
-  const int steps = (s.kbytes + kStep - 1) / kStep;
-  const int first = blockIdx.y * per, last = min(steps, first + per);
+  // the scales of the tile's rows and columns, on their way while it is
+  // computed
+  const int i0 = ti * BM, j0 = tj * BN, t = threadIdx.x;
+  float sx = 0.0f, sw = 0.0f, sb = 0.0f;
+  if (!slab && t < BM) {
+    sx = e.xs[min(i0 + t, s.rows_a - 1)];
+    sw = e.ws[min(j0 + t, s.rows_b - 1)];
+    if (e.bias) sb = e.bias[min(j0 + t, s.rows_b - 1)];
+  }
   v4i acc[P::MI][P::NJ];
-  P::run(s, ti * BM, tj * BN, 0, first, last, lds, acc);
+  P::run(s, i0, j0, 0, blockIdx.y, (s.kbytes + kStep - 1) / kStep, gridDim.y,
+         lds, acc);
+  float* scales = (float*)lds;
+  if (!slab) {
+    if (t < BM) {
+      scales[t] = sx;
+      scales[BM + t] = sw;
+      scales[2 * BM + t] = sb;
+    }
+    __syncthreads();
+  }
   int wm, wn;
   if (P::place(wm, wn)) return;
   const int lane = threadIdx.x & 63;
-  const int m0 = ti * BM + wm + (lane & 15);
-  const int n0 = tj * BN + wn + (lane >> 4) * 4;
+  const int m0 = wm + (lane & 15), n0 = wn + (lane >> 4) * 4;
 #pragma unroll
   for (int i = 0; i < P::MI; ++i) {
-    const long m = m0 + i * 16;
+    const long m = i0 + m0 + i * 16;
     if (m >= s.rows_a) continue;
 #pragma unroll
     for (int j = 0; j < P::NJ; ++j) {
-      const long n = n0 + j * 16;
+      const long n = j0 + n0 + j * 16;
       if (n >= s.rows_b) continue;
       if (slab) {
         int* to = slab + ((long)blockIdx.y * s.rows_a + m) * s.rows_b + n;
@@ -345,7 +372,9 @@ void int8_tile_k(
         for (int r = 0; r < 4; ++r)
           if (n + r < s.rows_b) to[r] = acc[i][j][r];
       } else {
-        store4<T>(e, m, n, acc[i][j]);
+        store4<T>(e, m, n, acc[i][j], scales[m0 + i * 16],
+                  *(const v4f*)(scales + BM + n0 + j * 16),
+                  *(const v4f*)(scales + 2 * BM + n0 + j * 16));
       }
     }
   }
@@ -353,10 +382,10 @@ void int8_tile_k(
 
 // Few rows of x (at most 16 MT): the weights' bytes are what counts. A wave
 // takes 16 output channels straight from memory to registers, no LDS; the
-// four waves of a workgroup, and gridDim.y workgroups, share out K.
+// four waves of a workgroup, and gridDim.y workgroups, take K's steps in turn.
 template <class T, int MT>
 __global__ __launch_bounds__(256) void int8_few_rows_k(
-    Sources s, Scales e, int per, int* __restrict__ slab) {
+    Sources s, Scales e, int* __restrict__ slab) {
   __shared__ v4i sums[4][MT][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -364,7 +393,7 @@ __global__ __launch_bounds__(256) void int8_few_rows_k(
   const int chunk = lane >> 4;
   const int steps = (s.kbytes + kStep - 1) / kStep;
   const int tail = s.kbytes - (steps - 1) * kStep;
-  const int first = blockIdx.y * per, last = min(steps, first + per);
+  const int stride = gridDim.y * 4;
   const char* pw = s.b[0] +
                    (long)min(n0 + (lane & 15), s.rows_b - 1) * s.row_b;
   const char* px[MT];
@@ -387,15 +416,16 @@ __global__ __launch_bounds__(256) void int8_few_rows_k(
         acc[t] = mma(w, *(const v4i*)(px[t] + at), acc[t]);
     }
   };
-  const bool mine = last == steps && tail < kStep;  // the cut step is here
-  const int whole = mine ? last - 1 : last;
-  int k = first + wave;
-  for (; k + 12 < whole; k += 16) {
+  const int whole = tail < kStep ? steps - 1 : steps;
+  int k = blockIdx.y * 4 + wave;
+  for (; k + 3 * stride < whole; k += 4 * stride) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) step(k + 4 * u, false);
+    for (int u = 0; u < 4; ++u) step(k + u * stride, false);
   }
-  for (; k < whole; k += 4) step(k, false);
-  if (mine && k == last - 1) step(k, true);
+  for (; k < whole; k += stride) step(k, false);
+  if (k < steps) step(k, true);
+  v4f ws, bias;
+  if (!slab) four_columns(e, n0 + chunk * 4, ws, bias);
 #pragma unroll
   for (int t = 0; t < MT; ++t) sums[wave][t][lane] = acc[t];
   __syncthreads();
@@ -411,7 +441,7 @@ __global__ __launch_bounds__(256) void int8_few_rows_k(
       for (int r = 0; r < 4; ++r)
         if (n + r < s.rows_b) to[r] = v[r];
     } else {
-      store4<T>(e, m, n, v);
+      store4<T>(e, m, n, v, e.xs[m], ws, bias);
     }
   }
 }
@@ -494,15 +524,15 @@ __global__ __launch_bounds__(256) void int8_linear_few_k(
       }
     }
   sums[wave][lane] = acc;
+  v4f ws, bias;
+  if (wave == 0) four_columns(e, n0 + chunk * 4, ws, bias);
   __syncthreads();
   if (wave == 0) {
 #pragma unroll
     for (int i = 1; i < 4; ++i) acc += sums[i][lane];
     const int row = lane & 15, n = n0 + chunk * 4;
     if (row < m && n < s.rows_b) {
-      Scales mine = e;
-      mine.xs = scale;
-      store4<T>(mine, row, n, acc);
+      store4<T>(e, row, n, acc, scale[row], ws, bias);
     }
   }
 }
@@ -521,8 +551,8 @@ __global__ __launch_bounds__(256) void int8_join_k(
 }
 
 // How a product is computed: by `rows` (16, 32 or 64) rows without LDS, or in
-// square tiles of `size`, each with K in `splits` parts of `per` steps.
-struct Plan { int rows, size, tm, tn, splits, per; };
+// square tiles of `size`, each with K's steps shared out over `splits`.
+struct Plan { int rows, size, tm, tn, splits; };
 
 Plan plan_of(long m, long n, long k) {
   Plan p = {};
@@ -534,13 +564,13 @@ Plan plan_of(long m, long n, long k) {
     p.tn = (int)((n + 15) / 16);
     long want = p.tn >= 512 ? 1 : (512 + p.tn - 1) / p.tn;
     want = std::min(want, std::min(64L, std::max(1L, (long)steps / 16)));
-    p.per = (int)((steps + want - 1) / want);
+    p.splits = (int)want;
   } else {
     // the tile and the split that need the least time; joining the parts
     // takes a launch, and writes and reads them at 4 TB/s
     double best = 1e30;
-    for (const TileCost& c : kTiles)
-      for (int splits = 1; splits <= 64 && splits * 4 <= steps + 3;
+    for (const TileCost& c : kTiles[0])
+      for (int splits = 1; splits <= 64 && splits <= (steps + 3) / 4;
            splits *= 2) {
         const long tm = (m + c.size - 1) / c.size;
         const long tn = (n + c.size - 1) / c.size;
@@ -553,11 +583,10 @@ Plan plan_of(long m, long n, long k) {
           p.size = c.size;
           p.tm = (int)tm;
           p.tn = (int)tn;
-          p.per = per;
+          p.splits = splits;
         }
       }
   }
-  p.splits = (steps + p.per - 1) / p.per;
   return p;
 }
 
@@ -567,16 +596,16 @@ void product(const Sources& s, const Scales& e, const Plan& p, int* slab,
   const dim3 grid(p.tm * p.tn, p.splits);
 #define FEW(MT)                                                           \
   hipLaunchKernelGGL((int8_few_rows_k<T, MT>), grid, dim3(256), 0, st, s, \
-                     e, p.per, slab)
-#define TILE(BM, WM, WN, STAGES, GROUPS)                                 \
+                     e, slab)
+#define TILE(BM, WM, WN, STAGES, GROUPS, PARTS)                          \
   hipLaunchKernelGGL((int8_tile_k<T, BM, WM, WN, STAGES, GROUPS>), grid, \
                      dim3(GROUPS * (BM / WM) * (BM / WN) * 64), 0, st,   \
-                     s, e, p.tm, p.tn, p.per, slab)
+                     s, e, p.tm, p.tn, slab)
   if (p.rows == 16) FEW(1);
   else if (p.rows == 32) FEW(2);
   else if (p.rows == 64) FEW(4);
   else {
-    BY_TILE_SIZE(p.size, (long)p.tm * p.tn * p.splits, TILE)
+    BY_TILE_SIZE_1(p.size, (long)p.tm * p.tn * p.splits, TILE)
   }
 #undef FEW
 #undef TILE

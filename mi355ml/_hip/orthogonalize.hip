@@ -750,10 +750,10 @@ __global__ __launch_bounds__(256) void split_k(
 // result.
 enum { kHalves, kFloat, kFp16, kBf16 };
 
-template <int OUT, int BM, int WM, int WN, int STAGES, int GROUPS>
+template <int OUT, int BM, int WM, int WN, int STAGES, int GROUPS, int PARTS>
 __global__ __launch_bounds__(GROUPS * (BM / WM) * (BM / WN) * 64)
 void step_k(Sources s, Step p) {
-  typedef Tile<v4f, BM, BM, WM, WN, STAGES, GROUPS> P;
+  typedef Tile<v4f, BM, BM, WM, WN, STAGES, GROUPS, PARTS> P;
   __shared__ __attribute__((aligned(16))) char lds[P::kLds];
   int ti, tj;
   const int b = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -762,7 +762,7 @@ void step_k(Sources s, Step p) {
   v4f acc[P::MI][P::NJ];
   const long z = blockIdx.y;
   P::run(s, ti * BM, tj * BM, z, 0,
-         s.parts * ((s.kbytes + kStep - 1) / kStep), lds, acc);
+         (PARTS > 1 ? 1 : s.parts) * (s.kbytes / kStep), 1, lds, acc);
   int wm0, wn0;
   if (P::place(wm0, wn0)) return;
   wm0 += ti * BM;
@@ -857,7 +857,7 @@ void step_k(Sources s, Step p) {
   }
 }
 
-template <int OUT>
+template <int OUT, int PARTS>
 void step_as(Sources s, Step p, int batch, hipStream_t st) {
   auto tiles_of = [&](int size) {
     const long tm = (s.rows_a + size - 1) / size;
@@ -866,9 +866,8 @@ void step_as(Sources s, Step p, int batch, hipStream_t st) {
   };
   int size = 0;
   double best = 0;
-  for (const TileCost& c : kTiles) {
-    const double t = tile_time(c, tiles_of(c.size) * batch,
-                               (long)s.parts * s.kbytes / kStep);
+  for (const TileCost& c : kTiles[PARTS - 1]) {
+    const double t = tile_time(c, tiles_of(c.size) * batch, s.kbytes / kStep);
     if (!size || t < best) {
       size = c.size;
       best = t;
@@ -877,10 +876,17 @@ void step_as(Sources s, Step p, int batch, hipStream_t st) {
   p.tm = (s.rows_a + size - 1) / size;
   p.tn = (s.rows_b + size - 1) / size;
   const dim3 grid((unsigned)tiles_of(size), batch);
-#define STEP(BM, WM, WN, STAGES, GROUPS)                              \
-  hipLaunchKernelGGL((step_k<OUT, BM, WM, WN, STAGES, GROUPS>), grid, \
+  const long tiles = tiles_of(size) * batch;
+#define STEP(BM, WM, WN, STAGES, GROUPS, TAKEN)                              \
+  hipLaunchKernelGGL((step_k<OUT, BM, WM, WN, STAGES, GROUPS, TAKEN>), grid, \
                      dim3(GROUPS * (BM / WM) * (BM / WN) * 64), 0, st, s, p)
-  BY_TILE_SIZE(size, tiles_of(size) * batch, STEP)
+  if constexpr (PARTS == 1) {
+    BY_TILE_SIZE_1(size, tiles, STEP)
+  } else if constexpr (PARTS == 2) {
+    BY_TILE_SIZE_2(size, tiles, STEP)
+  } else {
+    BY_TILE_SIZE_3(size, tiles, STEP)
+  }
 #undef STEP
 }
 
@@ -1064,7 +1070,8 @@ extern "C" void launch_split(const void* x, int dtype, int rows, int cols,
 #undef CALL
 }
 
-// a, b: the operands' hi and lo; parts 1: hi hi, 2: hi hi + hi lo, 3: all.
+// a, b: the operands' hi and lo; parts 1: hi hi, 2: hi hi + hi lo, 3: all. A
+// result in float32 or fp16 comes of three parts, one in bfloat16 of one.
 extern "C" void launch_step(Halves a, int rows_a, Halves b, int rows_b, int k,
                             int parts, Step p, int batch, int out,
                             hipStream_t st) {
@@ -1083,10 +1090,11 @@ extern "C" void launch_step(Halves a, int rows_a, Halves b, int rows_b, int k,
   s.rows_b = rows_b;
   s.kbytes = (k + 63) / 64 * 128;  // the filling is zeros
   s.parts = parts;
-  switch (out) {
-    case kHalves: step_as<kHalves>(s, p, batch, st); break;
-    case kFloat: step_as<kFloat>(s, p, batch, st); break;
-    case kFp16: step_as<kFp16>(s, p, batch, st); break;
-    default: step_as<kBf16>(s, p, batch, st);
-  }
+  // the combinations that by_products makes
+  if (out == kHalves && parts == 1) step_as<kHalves, 1>(s, p, batch, st);
+  else if (out == kHalves && parts == 2) step_as<kHalves, 2>(s, p, batch, st);
+  else if (out == kHalves) step_as<kHalves, 3>(s, p, batch, st);
+  else if (out == kFloat) step_as<kFloat, 3>(s, p, batch, st);
+  else if (out == kFp16) step_as<kFp16, 3>(s, p, batch, st);
+  else step_as<kBf16, 1>(s, p, batch, st);
 }

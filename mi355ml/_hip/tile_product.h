@@ -20,8 +20,10 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kStep = 128;  // bytes of K in one step
 
-// What a launch reads. `parts` pairs of operands are summed as if their K
-// were joined (a value split in two 16-bit halves takes two or three).
+// What a launch reads. Values that are held as two 16-bit numbers, hi + lo,
+// give two or three `parts` whose products are summed: (a, b)[0] hi hi, [1]
+// hi lo and [2] lo hi. A tile either takes them all in each step (PARTS > 1),
+// or one after the other, as if their K were joined (PARTS = 1).
 struct Sources {
   const char* a[3];
   const char* b[3];
@@ -86,20 +88,28 @@ template <int N> struct Count { static constexpr int value = N; };
 // half of them takes the second half of every step, and gives its sums to the
 // first at the end. That is for a CU's only workgroup, with one wave for each
 // SIMD otherwise (64 steps of a 64 x 64 tile 17.6 us, with one group 21.6).
+// PARTS = 2 or 3 takes hi and lo in the same step: three products for four
+// operands that are read, not six. Up to 128 x 128, which are bound by what
+// they read, that takes 0.6 to 0.85 of the time (1024^2 outputs, K = 2048,
+// three parts by 64: 15 us, joined 25; 2048^2 by 128: 48, joined 58). Larger
+// tiles do not have the LDS, and gain nothing by it.
 //
 // At 4096^3 a product of fp16 runs at 1.2 PFLOP/s and one of int8 at 2.6 POP/s
 // (the library: 1.1 and 2.05). There the matrix cores are busy 60% of the time
 // at a clock that the power limit holds at 1.75 GHz; LDS is at a quarter of
 // its rate. Small tiles are bound by what a CU takes in: a step of 64 x 64
 // is 16 KB in 520 clocks, of about 40 B a clock that loads alone reach.
-template <class ACC, int BM, int BN, int WM, int WN, int STAGES, int GROUPS>
+template <class ACC, int BM, int BN, int WM, int WN, int STAGES, int GROUPS,
+          int PARTS>
 struct Tile {
   static constexpr int kCols = BN / WN;
   static constexpr int kGroup = (BM / WM) * kCols;  // waves of a group
   static constexpr int kWaves = GROUPS * kGroup;
   static constexpr int kThreads = kWaves * 64;
   static constexpr int MI = WM / 16, NJ = WN / 16;
-  static constexpr int kStage = (BM + BN) * kStep;
+  static constexpr int PA = PARTS == 3 ? 2 : 1, PB = PARTS > 1 ? 2 : 1;
+  static constexpr int kRows = PA * BM + PB * BN;
+  static constexpr int kStage = kRows * kStep;
   static constexpr int kLds = STAGES * kStage;
   static constexpr bool kInt = __is_same(ACC, v4i);
 
@@ -108,7 +118,8 @@ struct Tile {
   // reads behind the multiplications and then waits for them.
   template <int V>
   static __device__ __forceinline__ void interleave() {
-    constexpr int R = MI + NJ, M = MI * NJ, EACH = M / (R + V);
+    constexpr int R = PA * MI + PB * NJ, M = MI * NJ * PARTS;
+    constexpr int EACH = M / (R + V);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
@@ -133,31 +144,35 @@ struct Tile {
   // acc[i][j][r] is the sum for row  m = i * 16 + lane % 16  and column
   // n = j * 16 + lane / 16 * 4 + r  of the wave's part of the tile: B goes in
   // as the first operand, so that a lane ends with four columns side by side.
+  //
+  // Steps first, first + stride, ... before last; a stride other than 1 is
+  // for one part alone.
   static __device__ __forceinline__ void run(const Sources& s, int m0, int n0,
                                              long batch, int first, int last,
-                                             char* lds,
+                                             int stride, char* lds,
                                              ACC (&acc)[MI][NJ]) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int group = wave / kGroup;
     const int wm = wave % kGroup / kCols, wn = wave % kCols;
     // the wave's share of the rows to load, 8 at a time, A's before B's
-    constexpr int LOADS = (BM + BN) / 8 / kWaves;
-    static_assert(LOADS * kWaves * 8 == BM + BN, "");
+    constexpr int LOADS = kRows / 8 / kWaves;
+    static_assert(LOADS * kWaves * 8 == kRows, "");
     const int r8 = lane >> 3;
     const int c16 = ((lane & 7) ^ r8) * 16;
     // rows behind the last are read from the last one; nothing is stored
     // from what they give
     unsigned at_row[LOADS];
-    bool of_a[LOADS];
+    int plane[LOADS];
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
       const int r = (u * kWaves + wave) * 8;
-      of_a[u] = r < BM;
-      at_row[u] =
-          of_a[u]
-              ? (unsigned)(min(m0 + r + r8, s.rows_a - 1) - m0) * s.row_a
-              : (unsigned)(min(n0 + r - BM + r8, s.rows_b - 1) - n0) * s.row_b;
+      const bool of_a = r < PA * BM;
+      const int rr = of_a ? r % BM : (r - PA * BM) % BN;
+      plane[u] = of_a ? r / BM : 2 + (r - PA * BM) / BN;
+      at_row[u] = of_a
+                      ? (unsigned)(min(m0 + rr + r8, s.rows_a - 1) - m0) * s.row_a
+                      : (unsigned)(min(n0 + rr + r8, s.rows_b - 1) - n0) * s.row_b;
     }
     const int steps = (s.kbytes + kStep - 1) / kStep;
     const int tail = s.kbytes - (steps - 1) * kStep;  // bytes of the last step
@@ -165,9 +180,11 @@ struct Tile {
     const long at_b = batch * s.batch_b + (long)n0 * s.row_b;
 
     // where the next step is loaded from
-    const char* pa = s.a[0] + at_a + (long)(first % steps) * kStep;
-    const char* pb = s.b[0] + at_b + (long)(first % steps) * kStep;
-    int k = first % steps, part = 0;
+    const char* pa = s.a[0] + at_a + (long)first * kStep;
+    const char* pb = s.b[0] + at_b + (long)first * kStep;
+    const long lo_a = PA == 2 ? s.a[2] - s.a[0] : 0;
+    const long lo_b = PB == 2 ? s.b[1] - s.b[0] : 0;
+    int k = first, part = 0;
     // from the end of one part to the beginning of the next
     const long back = (long)steps * kStep - kStep;
     const long a1 = s.a[1] - s.a[0] - back, a2 = s.a[2] - s.a[1] - back;
@@ -181,35 +198,46 @@ struct Tile {
       for (int u = 0; u < LOADS; ++u)
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) void*)(
-                (of_a[u] ? pa : pb) + (at_row[u] + c)),
+                (plane[u] == 0   ? pa
+                 : plane[u] == 1 ? pa + lo_a
+                 : plane[u] == 2 ? pb
+                                 : pb + lo_b) +
+                (at_row[u] + c)),
             (__attribute__((address_space(3))) void*)(to + u * kWaves * 1024),
             16, 0, 0);
-      const bool wrap = ++k == steps;
+      k += stride;
+      const bool wrap = PARTS == 1 && !kInt && k == steps;
       k = wrap ? 0 : k;
-      pa += wrap ? (part ? a2 : a1) : (long)kStep;
-      pb += wrap ? (part ? b2 : b1) : (long)kStep;
+      pa += wrap ? (part ? a2 : a1) : (long)stride * kStep;
+      pb += wrap ? (part ? b2 : b1) : (long)stride * kStep;
       part += wrap;
     };
     const char* base_a = lds + (wm * WM + (lane & 15)) * kStep;
-    const char* base_b = lds + (BM + wn * WN + (lane & 15)) * kStep;
+    const char* base_b = lds + (PA * BM + wn * WN + (lane & 15)) * kStep;
     // 64 bytes of each row: one operand of each matrix instruction
-    struct Half { v4i a[MI], b[NJ]; };
+    struct Half { v4i a[PA][MI], b[PB][NJ]; };
     auto fetch = [&](Half& f, int buf, int kk) {
       const int at = buf * kStage +
                      ((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 16;
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
-        f.a[i] = *(const v4i*)(base_a + at + i * 16 * kStep);
+      for (int p = 0; p < PA; ++p)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        f.b[j] = *(const v4i*)(base_b + at + j * 16 * kStep);
+        for (int i = 0; i < MI; ++i)
+          f.a[p][i] = *(const v4i*)(base_a + at + (p * BM + i * 16) * kStep);
+#pragma unroll
+      for (int p = 0; p < PB; ++p)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          f.b[p][j] = *(const v4i*)(base_b + at + (p * BN + j * 16) * kStep);
     };
     auto multiply = [&](const Half& f) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+      for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-          acc[i][j] = mma(f.b[j], f.a[i], acc[i][j]);
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            acc[i][j] = mma(f.b[p == 1][j], f.a[p == 2][i], acc[i][j]);
     };
     // All loads but the last N steps' are in, and every wave is done with
     // the buffer of the step before.
@@ -238,7 +266,7 @@ struct Tile {
     // wait for nothing but the barrier (one a step). A buffer is loaded again
     // right after the turn that frees it.
     Half f0, f1;
-    const int count = last - first;
+    const int count = (last - first + stride - 1) / stride;
 #pragma unroll
     for (int u = 0; u < STAGES; ++u)
       if (u < count) load(u);
@@ -251,9 +279,10 @@ struct Tile {
     auto cut = [&](Half& f, int from) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
-        f.b[j] = keep_bytes(f.b[j], tail - from - (lane >> 4) * 16);
+        f.b[0][j] = keep_bytes(f.b[0][j], tail - from - (lane >> 4) * 16);
     };
-    const bool ragged = kInt && tail < kStep && last % steps == 0;
+    const bool ragged = kInt && tail < kStep &&
+                        first + (count - 1) * stride == steps - 1;
     if constexpr (GROUPS == 1) {
       for (; t + STAGES < count; ++t) {
         fetch(f1, buf, 1);
@@ -338,9 +367,15 @@ struct TileCost {
   int size;
   double first, more, ends;
 };
-constexpr TileCost kTiles[] = {
-    {256, 1.75, 1.75, 20.0}, {192, 1.0, 1.1, 11.0}, {128, 0.6, 0.57, 4.5},
-    {96, 0.41, 0.37, 2.8},   {64, 0.28, 0.21, 1.3}, {32, 0.2, 0.1, 0.5}};
+constexpr int kSizes = 6;
+// by the parts of a product
+constexpr TileCost kTiles[3][kSizes] = {
+    {{256, 1.75, 1.75, 20.0}, {192, 1.0, 1.1, 11.0}, {128, 0.6, 0.57, 4.5},
+     {96, 0.41, 0.37, 2.8}, {64, 0.28, 0.21, 1.3}, {32, 0.2, 0.1, 0.5}},
+    {{256, 3.5, 3.5, 20.0}, {192, 2.0, 2.2, 11.0}, {128, 0.91, 1.0, 4.5},
+     {96, 0.79, 0.63, 2.8}, {64, 0.34, 0.34, 1.3}, {32, 0.26, 0.14, 0.5}},
+    {{256, 5.4, 5.4, 20.0}, {192, 3.0, 3.3, 11.0}, {128, 1.5, 1.5, 4.5},
+     {96, 0.92, 0.87, 2.8}, {64, 0.47, 0.43, 1.3}, {32, 0.32, 0.17, 0.5}}};
 
 // us for `tiles` tiles of `steps` steps
 inline double tile_time(const TileCost& c, long tiles, long steps) {
@@ -350,28 +385,54 @@ inline double tile_time(const TileCost& c, long tiles, long steps) {
   return step * steps + c.ends * rounds;
 }
 
-// LAUNCH(BM, WM, WN, STAGES, GROUPS) for tiles of `size`. Up to 128, where a
-// CU gets one tile at most, four steps in LDS are quicker (2048^2 outputs by
-// 128: 39 us for 64 steps, with two 47), otherwise two, so that several
-// workgroups fit (4096^2 by 128: 144 us, with four 159).
-#define BY_TILE_SIZE(size, tiles, LAUNCH)          \
-  const bool alone = (tiles) <= 256;               \
-  switch (size) {                                  \
-    case 256: LAUNCH(256, 128, 64, 2, 1); break;   \
-    case 192: LAUNCH(192, 96, 48, 3, 1); break;    \
-    case 128:                                      \
-      if (alone) LAUNCH(128, 64, 32, 4, 1);        \
-      else LAUNCH(128, 64, 32, 2, 1);              \
-      break;                                       \
-    case 96:                                       \
-      if (alone) LAUNCH(96, 48, 48, 4, 2);         \
-      else LAUNCH(96, 48, 48, 2, 1);               \
-      break;                                       \
-    case 64:                                       \
-      if (alone) LAUNCH(64, 32, 32, 4, 2);         \
-      else LAUNCH(64, 32, 32, 2, 1);               \
-      break;                                       \
-    default: LAUNCH(32, 16, 16, 4, 1);             \
+// LAUNCH(BM, WM, WN, STAGES, GROUPS, PARTS) for tiles of `size`. Up to 128,
+// where a CU gets one tile at most, as many steps in LDS as fit are quicker
+// (2048^2 outputs by 128: 39 us for 64 steps, with two 47), otherwise two, so
+// that several workgroups fit (4096^2 by 128: 144 us, with four 159).
+#define BY_TILE_SIZE_1(size, tiles, LAUNCH)               \
+  switch (size) {                                         \
+    case 256: LAUNCH(256, 128, 64, 2, 1, 1); break;       \
+    case 192: LAUNCH(192, 96, 48, 3, 1, 1); break;        \
+    case 128:                                             \
+      if ((tiles) <= 256) LAUNCH(128, 64, 32, 4, 1, 1);   \
+      else LAUNCH(128, 64, 32, 2, 1, 1);                  \
+      break;                                              \
+    case 96:                                              \
+      if ((tiles) <= 256) LAUNCH(96, 48, 48, 4, 2, 1);    \
+      else LAUNCH(96, 48, 48, 2, 1, 1);                   \
+      break;                                              \
+    case 64:                                              \
+      if ((tiles) <= 256) LAUNCH(64, 32, 32, 4, 2, 1);    \
+      else LAUNCH(64, 32, 32, 2, 1, 1);                   \
+      break;                                              \
+    default: LAUNCH(32, 16, 16, 4, 1, 1);                 \
+  }
+#define BY_TILE_SIZE_2(size, tiles, LAUNCH)               \
+  switch (size) {                                         \
+    case 256: LAUNCH(256, 128, 64, 2, 1, 1); break;       \
+    case 192: LAUNCH(192, 96, 48, 3, 1, 1); break;        \
+    case 128: LAUNCH(128, 64, 32, 3, 1, 2); break;        \
+    case 96:                                              \
+      if ((tiles) <= 256) LAUNCH(96, 48, 48, 4, 1, 2);    \
+      else LAUNCH(96, 48, 48, 2, 1, 2);                   \
+      break;                                              \
+    case 64:                                              \
+      if ((tiles) <= 256) LAUNCH(64, 32, 32, 4, 2, 2);    \
+      else LAUNCH(64, 32, 32, 2, 1, 2);                   \
+      break;                                              \
+    default: LAUNCH(32, 16, 16, 4, 1, 2);                 \
+  }
+#define BY_TILE_SIZE_3(size, tiles, LAUNCH)               \
+  switch (size) {                                         \
+    case 256: LAUNCH(256, 128, 64, 2, 1, 1); break;       \
+    case 192: LAUNCH(192, 96, 48, 3, 1, 1); break;        \
+    case 128: LAUNCH(128, 64, 32, 2, 1, 3); break;        \
+    case 96: LAUNCH(96, 48, 48, 3, 2, 3); break;          \
+    case 64:                                              \
+      if ((tiles) <= 256) LAUNCH(64, 32, 32, 4, 2, 3);    \
+      else LAUNCH(64, 32, 32, 2, 2, 3);                   \
+      break;                                              \
+    default: LAUNCH(32, 16, 16, 4, 1, 3);                 \
   }
 
 }  // namespace tile_product

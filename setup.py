@@ -14,6 +14,16 @@ os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
 
 from torch.utils.cpp_extension import BuildExtension, CUDAExtension  # noqa: E402
 
+# The build does not see which headers a .hip or .cpp file includes: a file
+# that is older than one of them is marked as changed.
+_hip = os.path.join(os.path.dirname(os.path.abspath(__file__)), "mi355ml",
+                    "_hip")
+_files = [os.path.join(_hip, f) for f in os.listdir(_hip)]
+_newest = max(os.path.getmtime(f) for f in _files if f.endswith(".h"))
+for _f in _files:
+    if not _f.endswith(".h") and os.path.getmtime(_f) < _newest:
+        os.utime(_f)
+
 ext = CUDAExtension(
     name="mi355ml._hip_ext",
     sources=[
