@@ -290,16 +290,44 @@ template <class T> __device__ __forceinline__ T narrow(float v) {
   return (T)v;
 }
 
-// Four columns side by side of one row: y = acc xs ws + bias, rounded once.
+// y = acc xs ws + bias for four columns side by side, rounded once.
+template <class T>
+__device__ __forceinline__ void scaled(const v4i& acc, float xs, const v4f& ws,
+                                       const v4f& bias, T (&v)[4]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    v[r] = narrow<T>(fmaf((float)acc[r] * xs, ws[r], bias[r]));
+}
+
+// 16 bytes from LDS to a row's values from `at` on, as far as it goes.
+template <class T>
+__device__ __forceinline__ void store_piece(T* row, bool here, long at, long n,
+                                            const char* from) {
+  constexpr int N = 16 / sizeof(T);
+  if (!here || at >= n) return;
+  struct __attribute__((aligned(16))) Whole { T v[N]; };
+  struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[N]; };
+  const Whole w = *(const Whole*)from;
+  if (at + N <= n) {
+    Raw raw;
+#pragma unroll
+    for (int e = 0; e < N; ++e) raw.v[e] = w.v[e];
+    *(Raw*)(row + at) = raw;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (at + e < n) row[at + e] = w.v[e];
+  }
+}
+
+// Four columns of one row, by a lane on its own.
 template <class T>
 __device__ __forceinline__ void store4(const Scales& e, long m, long n,
                                        const v4i& acc, float xs, const v4f& ws,
                                        const v4f& bias) {
   T* out = (T*)e.out + m * e.n + n;
   T v[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    v[r] = narrow<T>(fmaf((float)acc[r] * xs, ws[r], bias[r]));
+  scaled<T>(acc, xs, ws, bias, v);
   if (e.vec && n + 4 <= e.n) {
     struct __attribute__((aligned(4 * sizeof(T)))) Four { T v[4]; };
     *(Four*)out = Four{v[0], v[1], v[2], v[3]};
@@ -345,39 +373,43 @@ void int8_tile_k(
   v4i acc[P::MI][P::NJ];
   P::run(s, i0, j0, 0, blockIdx.y, (s.kbytes + kStep - 1) / kStep, gridDim.y,
          lds, acc);
-  float* scales = (float*)lds;
-  if (!slab) {
-    if (t < BM) {
-      scales[t] = sx;
-      scales[BM + t] = sw;
-      scales[2 * BM + t] = sb;
-    }
-    __syncthreads();
-  }
   int wm, wn;
-  if (P::place(wm, wn)) return;
+  const bool mine = !P::place(wm, wn);
   const int lane = threadIdx.x & 63;
-  const int m0 = wm + (lane & 15), n0 = wn + (lane >> 4) * 4;
+  if (slab) {
+    typedef Rows<P, BM, BN, int, 1, false> R;
+    R::store(lds, mine, wm, wn,
+             [&](int i, int j, int (&v)[1][4]) {
 #pragma unroll
-  for (int i = 0; i < P::MI; ++i) {
-    const long m = i0 + m0 + i * 16;
-    if (m >= s.rows_a) continue;
-#pragma unroll
-    for (int j = 0; j < P::NJ; ++j) {
-      const long n = j0 + n0 + j * 16;
-      if (n >= s.rows_b) continue;
-      if (slab) {
-        int* to = slab + ((long)blockIdx.y * s.rows_a + m) * s.rows_b + n;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < s.rows_b) to[r] = acc[i][j][r];
-      } else {
-        store4<T>(e, m, n, acc[i][j], scales[m0 + i * 16],
-                  *(const v4f*)(scales + BM + n0 + j * 16),
-                  *(const v4f*)(scales + 2 * BM + n0 + j * 16));
-      }
-    }
+               for (int r = 0; r < 4; ++r) v[0][r] = acc[i][j][r];
+             },
+             [&](int, int row, int column, const char* at) {
+               store_piece<int>(slab + ((long)blockIdx.y * s.rows_a + i0 +
+                                        row) * s.rows_b,
+                                i0 + row < s.rows_a, j0 + column, s.rows_b,
+                                at);
+             });
+    return;
   }
+  typedef Rows<P, BM, BN, T, 1, false> R;
+  static_assert(R::kLds + 3 * BM * 4 <= P::kLds, "");
+  float* scales = (float*)(lds + R::kLds);
+  if (t < BM) {
+    scales[t] = sx;
+    scales[BM + t] = sw;
+    scales[2 * BM + t] = sb;
+  }
+  const int m0 = wm + (lane & 15), n0 = wn + (lane >> 4) * 4;
+  R::store(lds, mine, wm, wn,
+           [&](int i, int j, T (&v)[1][4]) {
+             scaled<T>(acc[i][j], scales[m0 + i * 16],
+                       *(const v4f*)(scales + BM + n0 + j * 16),
+                       *(const v4f*)(scales + 2 * BM + n0 + j * 16), v[0]);
+           },
+           [&](int, int row, int column, const char* at) {
+             store_piece<T>((T*)e.out + (long)(i0 + row) * e.n,
+                            i0 + row < s.rows_a, j0 + column, s.rows_b, at);
+           });
 }
 
 // Few rows of x (at most 16 MT): the weights' bytes are what counts. A wave

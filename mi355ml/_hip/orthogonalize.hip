@@ -27,6 +27,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "orthogonalize.h"
 #include "tile_product.h"
 
@@ -763,97 +765,106 @@ void step_k(Sources s, Step p) {
   const long z = blockIdx.y;
   P::run(s, ti * BM, tj * BM, z, 0,
          (PARTS > 1 ? 1 : s.parts) * (s.kbytes / kStep), 1, lds, acc);
-  int wm0, wn0;
-  if (P::place(wm0, wn0)) return;
-  wm0 += ti * BM;
-  wn0 += tj * BM;
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  const int c = lane & 15, h = lane >> 4;
+  int wm, wn;
+  const bool mine = !P::place(wm, wn);
+  const int lane = threadIdx.x & 63, c = lane & 15, h = lane >> 4;
+  const int i0 = ti * BM, j0 = tj * BM;
   const int rows = s.rows_a, cols = s.rows_b;
   float alpha = p.alpha;
   if (p.power) alpha *= p.factor[z];
   if (p.power == 2) alpha *= p.factor[z];
   const float ungain = 1.0f / p.gain;
-  // the wave's own piece of LDS: 16 columns of its part, for storing along
-  // the other side
-  constexpr int LD = WM + 8;
-  _Float16* th = (_Float16*)lds + wave * (2 * 16 * LD);
-  _Float16* tl = th + 16 * LD;
-  const bool across = OUT == kHalves && p.t.hi && !(p.symmetric && ti == tj);
 #pragma unroll
-  for (int j = 0; j < P::NJ; ++j) {
-    const int n = wn0 + j * 16 + h * 4;
+  for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-    for (int i = 0; i < P::MI; ++i) {
-      const int m = wm0 + i * 16 + c;
-      float v[4];
+    for (int j = 0; j < P::NJ; ++j) {
+      const int m = i0 + wm + i * 16 + c, n = j0 + wn + j * 16 + h * 4;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = alpha * acc[i][j][r];
-      if (p.e.hi && m < rows && n < cols) {
+      for (int r = 0; r < 4; ++r) acc[i][j][r] *= alpha;
+      if (OUT == kHalves && p.e.hi && mine && m < rows && n < cols) {
         const long at = z * p.e.batch + (long)m * p.e.ld + n;
         const v4h eh = *(const v4h*)(p.e.hi + at);
         const v4h el = *(const v4h*)(p.e.lo + at);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          v[r] += p.beta * ((float)eh[r] + (float)el[r] * ungain);
-          if (m == n + r) v[r] += p.diagonal;
+          acc[i][j][r] += p.beta * ((float)eh[r] + (float)el[r] * ungain);
+          if (m == n + r) acc[i][j][r] += p.diagonal;
         }
       }
-      if (OUT == kHalves) {
-        v4h hi, lo;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          // rows and columns that are not there count as zeros later
-          if (m >= rows || n + r >= cols) v[r] = 0.0f;
-          hi[r] = (_Float16)v[r];
-          lo[r] = (_Float16)((v[r] - (float)hi[r]) * p.gain);
-        }
-        if (p.d.hi && m < rows && n < cols) {
-          const long at = z * p.d.batch + (long)m * p.d.ld + n;
-          *(v4h*)(p.d.hi + at) = hi;
-          if (p.d.lo) *(v4h*)(p.d.lo + at) = lo;
-        }
-        if (across) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            th[(h * 4 + r) * LD + i * 16 + c] = hi[r];
-            tl[(h * 4 + r) * LD + i * 16 + c] = lo[r];
-          }
-        }
-      } else if (m < rows) {
-        const long step = p.tall ? p.ld_out : 1;
-        const long at = z * p.batch_out +
-                        (p.tall ? n * p.ld_out + m : m * p.ld_out + n);
+      // rows and columns that are not there count as zeros later
+      if (OUT == kHalves)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (n + r < cols) {
-            if (OUT == kFloat) ((float*)p.out)[at + r * step] = v[r];
-            else if (OUT == kFp16)
-              ((_Float16*)p.out)[at + r * step] = (_Float16)v[r];
-            else ((__bf16*)p.out)[at + r * step] = (__bf16)v[r];
-          }
-      }
+          if (m >= rows || n + r >= cols) acc[i][j][r] = 0.0f;
     }
-    if (across) {
-      // a wave's own writes and reads of LDS go in order; the compiler has to
-      // keep them so
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  if constexpr (OUT == kHalves) {
+    auto halves = [&](int i, int j, _Float16 (&v)[2][4]) {
 #pragma unroll
-      for (int u = 0; u < (16 * (WM / 8) + 63) / 64; ++u) {
-        const int k = u * 64 + lane;
-        if (k >= 16 * (WM / 8)) continue;
-        const int row = k / (WM / 8), m = wm0 + k % (WM / 8) * 8;
-        const int nn = wn0 + j * 16 + row;
-        if (nn < cols && m < rows) {
-          const long at = z * p.t.batch + (long)nn * p.t.ld + m;
-          *(v8h*)(p.t.hi + at) = *(const v8h*)(th + row * LD + m - wm0);
-          if (p.t.lo)
-            *(v8h*)(p.t.lo + at) = *(const v8h*)(tl + row * LD + m - wm0);
-        }
+      for (int r = 0; r < 4; ++r) {
+        v[0][r] = (_Float16)acc[i][j][r];
+        v[1][r] = (_Float16)((acc[i][j][r] - (float)v[0][r]) * p.gain);
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
+    };
+    // a row's filling goes to the next multiple of 64: eight values at a time
+    // end there at the latest
+    if (p.d.hi)
+      Rows<P, BM, BM, _Float16, 2, false>::store(
+          lds, mine, wm, wn, halves,
+          [&](int plane, int row, int column, const char* from) {
+            const int m = i0 + row, n = j0 + column;
+            unsigned short* to = plane ? p.d.lo : p.d.hi;
+            if (to && m < rows && n < cols)
+              *(v8h*)(to + z * p.d.batch + (long)m * p.d.ld + n) =
+                  *(const v8h*)from;
+          });
+    if (p.t.hi && !(p.symmetric && ti == tj))
+      Rows<P, BM, BM, _Float16, 2, true>::store(
+          lds, mine, wm, wn, halves,
+          [&](int plane, int row, int column, const char* from) {
+            const int m = i0 + column, n = j0 + row;
+            unsigned short* to = plane ? p.t.lo : p.t.hi;
+            if (to && m < rows && n < cols)
+              *(v8h*)(to + z * p.t.batch + (long)n * p.t.ld + m) =
+                  *(const v8h*)from;
+          });
+  } else {
+    typedef std::conditional_t<
+        OUT == kFloat, float,
+        std::conditional_t<OUT == kFp16, _Float16, __bf16>> T;
+    constexpr int N = 16 / sizeof(T);
+    struct __attribute__((aligned(16))) Whole { T v[N]; };
+    T* out = (T*)p.out + z * p.batch_out;
+    auto values = [&](int i, int j, T (&v)[1][4]) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[0][r] = (T)acc[i][j][r];
+    };
+    auto put = [&](long row, long most, long at, long n, const char* from) {
+      if (row >= most || at >= n) return;
+      const Whole w = *(const Whole*)from;
+      T* to = out + row * p.ld_out + at;
+      if (at + N <= n) {
+        typename Some<T, N>::Raw raw;
+#pragma unroll
+        for (int e = 0; e < N; ++e) raw.v[e] = w.v[e];
+        *(typename Some<T, N>::Raw*)to = raw;
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (at + e < n) to[e] = w.v[e];
+      }
+    };
+    if (p.tall)
+      Rows<P, BM, BM, T, 1, true>::store(
+          lds, mine, wm, wn, values,
+          [&](int, int row, int column, const char* from) {
+            put(j0 + row, cols, i0 + column, rows, from);
+          });
+    else
+      Rows<P, BM, BM, T, 1, false>::store(
+          lds, mine, wm, wn, values,
+          [&](int, int row, int column, const char* from) {
+            put(i0 + row, rows, j0 + column, cols, from);
+          });
   }
 }
 
