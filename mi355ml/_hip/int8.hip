@@ -299,27 +299,6 @@ __device__ __forceinline__ void scaled(const v4i& acc, float xs, const v4f& ws,
     v[r] = narrow<T>(fmaf((float)acc[r] * xs, ws[r], bias[r]));
 }
 
-// 16 bytes from LDS to a row's values from `at` on, as far as it goes.
-template <class T>
-__device__ __forceinline__ void store_piece(T* row, bool here, long at, long n,
-                                            const char* from) {
-  constexpr int N = 16 / sizeof(T);
-  if (!here || at >= n) return;
-  struct __attribute__((aligned(16))) Whole { T v[N]; };
-  struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[N]; };
-  const Whole w = *(const Whole*)from;
-  if (at + N <= n) {
-    Raw raw;
-#pragma unroll
-    for (int e = 0; e < N; ++e) raw.v[e] = w.v[e];
-    *(Raw*)(row + at) = raw;
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (at + e < n) row[at + e] = w.v[e];
-  }
-}
-
 // Four columns of one row, by a lane on its own.
 template <class T>
 __device__ __forceinline__ void store4(const Scales& e, long m, long n,
@@ -359,6 +338,7 @@ void int8_tile_k(
   constexpr int BN = BM;
   typedef Tile<v4i, BM, BN, WM, WN, STAGES, GROUPS, 1> P;
   __shared__ __attribute__((aligned(16))) char lds[P::kLds];
+  __shared__ __attribute__((aligned(16))) float scales[3 * BM];
   int ti, tj;
   banded(xcd_contiguous(blockIdx.x, gridDim.x), tm, tn, ti, tj);
   // the scales of the tile's rows and columns, on their way while it is
@@ -392,8 +372,6 @@ void int8_tile_k(
     return;
   }
   typedef Rows<P, BM, BN, T, 1, false> R;
-  static_assert(R::kLds + 3 * BM * 4 <= P::kLds, "");
-  float* scales = (float*)(lds + R::kLds);
   if (t < BM) {
     scales[t] = sx;
     scales[BM + t] = sw;
@@ -481,16 +459,17 @@ __global__ __launch_bounds__(256) void int8_few_rows_k(
 // The same for rows of x that are still floats, and few values altogether:
 // every workgroup quantises them for itself into LDS, which takes less time
 // than a launch of its own, while its first weights are on their way.
-constexpr int kFewValues = 16384;  // m * k, both rounded up (16 rows)
+constexpr int kFewValues = 16384;  // m * k, k rounded up
+constexpr int kLinearWaves = 8;
 
 template <class TX, class T>
-__global__ __launch_bounds__(256) void int8_linear_few_k(
+__global__ __launch_bounds__(kLinearWaves * 64) void int8_linear_few_k(
     const TX* __restrict__ x, long stride, Sources s, Scales e) {
   constexpr int VEC = 16 / sizeof(TX);
   __shared__ __attribute__((aligned(16))) char rows[kFewValues + 16 * 16];
-  __shared__ float part[16][4];
+  __shared__ float part[16][kLinearWaves];
   __shared__ float scale[16];
-  __shared__ v4i sums[4][64];
+  __shared__ v4i sums[kLinearWaves][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = s.rows_a, k = s.kbytes;
@@ -512,10 +491,10 @@ __global__ __launch_bounds__(256) void int8_linear_few_k(
   for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
-      w[u][kk] = weights(min(wave + 4 * u, steps - 1), kk);
+      w[u][kk] = weights(min(wave + kLinearWaves * u, steps - 1), kk);
   for (int r = 0; r < m; ++r) {
     float big = 0.0f, v[VEC];
-    for (int at = threadIdx.x * VEC; at < k; at += 256 * VEC) {
+    for (int at = threadIdx.x * VEC; at < k; at += kLinearWaves * 64 * VEC) {
       load_chunk<TX, VEC>(x + r * stride, at, k, v);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) big = max_abs(big, v[i]);
@@ -528,10 +507,10 @@ __global__ __launch_bounds__(256) void int8_linear_few_k(
   for (int r = 0; r < m; ++r) {
     float big = part[r][0];
 #pragma unroll
-    for (int i = 1; i < 4; ++i) big = max_abs(big, part[r][i]);
+    for (int i = 1; i < kLinearWaves; ++i) big = max_abs(big, part[r][i]);
     const RowScale rs(big);
     if (threadIdx.x == 0) scale[r] = rs.scale();
-    for (int at = threadIdx.x * VEC; at < steps * 128; at += 256 * VEC) {
+    for (int at = threadIdx.x * VEC; at < steps * 128; at += kLinearWaves * 64 * VEC) {
       float v[VEC];
       uint32_t q[VEC / 4];
       load_chunk<TX, VEC>(x + r * stride, at, k, v);
@@ -544,15 +523,15 @@ __global__ __launch_bounds__(256) void int8_linear_few_k(
   __syncthreads();
   const char* px = rows + min(lane & 15, m - 1) * ld + chunk * 16;
   v4i acc = {0, 0, 0, 0};
-  for (int t = wave; t < steps; t += 4 * AHEAD)
+  for (int t = wave; t < steps; t += kLinearWaves * AHEAD)
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int at = t + 4 * u;
+      const int at = t + kLinearWaves * u;
       if (at >= steps) break;
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         acc = mma(w[u][kk], *(const v4i*)(px + at * 128 + kk * 64), acc);
-        w[u][kk] = weights(min(at + 4 * AHEAD, steps - 1), kk);
+        w[u][kk] = weights(min(at + kLinearWaves * AHEAD, steps - 1), kk);
       }
     }
   sums[wave][lane] = acc;
@@ -561,7 +540,7 @@ __global__ __launch_bounds__(256) void int8_linear_few_k(
   __syncthreads();
   if (wave == 0) {
 #pragma unroll
-    for (int i = 1; i < 4; ++i) acc += sums[i][lane];
+    for (int i = 1; i < kLinearWaves; ++i) acc += sums[i][lane];
     const int row = lane & 15, n = n0 + chunk * 4;
     if (row < m && n < s.rows_b) {
       store4<T>(e, row, n, acc, scale[row], ws, bias);
@@ -715,7 +694,8 @@ extern "C" void launch_int8_linear(const void* x, int xtype, long xstride,
   Scales e = {nullptr, ws, bias, out, n, n % 4 == 0};
   const dim3 grid((unsigned)((n + 15) / 16));
 #define FEW(TX, T)                                                        \
-  hipLaunchKernelGGL((int8_linear_few_k<TX, T>), grid, dim3(256), 0, st, \
+  hipLaunchKernelGGL((int8_linear_few_k<TX, T>), grid,                   \
+                     dim3(kLinearWaves * 64), 0, st,                     \
                      (const TX*)x, xstride, s, e)
 #define FEW_OUT(TX)                           \
   if (dtype == 0) FEW(TX, float);             \

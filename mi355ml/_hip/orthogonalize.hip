@@ -831,39 +831,24 @@ void step_k(Sources s, Step p) {
     typedef std::conditional_t<
         OUT == kFloat, float,
         std::conditional_t<OUT == kFp16, _Float16, __bf16>> T;
-    constexpr int N = 16 / sizeof(T);
-    struct __attribute__((aligned(16))) Whole { T v[N]; };
     T* out = (T*)p.out + z * p.batch_out;
     auto values = [&](int i, int j, T (&v)[1][4]) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[0][r] = (T)acc[i][j][r];
     };
-    auto put = [&](long row, long most, long at, long n, const char* from) {
-      if (row >= most || at >= n) return;
-      const Whole w = *(const Whole*)from;
-      T* to = out + row * p.ld_out + at;
-      if (at + N <= n) {
-        typename Some<T, N>::Raw raw;
-#pragma unroll
-        for (int e = 0; e < N; ++e) raw.v[e] = w.v[e];
-        *(typename Some<T, N>::Raw*)to = raw;
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (at + e < n) to[e] = w.v[e];
-      }
-    };
     if (p.tall)
       Rows<P, BM, BM, T, 1, true>::store(
           lds, mine, wm, wn, values,
           [&](int, int row, int column, const char* from) {
-            put(j0 + row, cols, i0 + column, rows, from);
+            store_piece<T>(out + (j0 + row) * p.ld_out, j0 + row < cols,
+                           i0 + column, rows, from);
           });
     else
       Rows<P, BM, BM, T, 1, false>::store(
           lds, mine, wm, wn, values,
           [&](int, int row, int column, const char* from) {
-            put(i0 + row, rows, j0 + column, cols, from);
+            store_piece<T>(out + (i0 + row) * p.ld_out, i0 + row < rows,
+                           j0 + column, cols, from);
           });
   }
 }

@@ -357,10 +357,31 @@ struct Tile {
   }
 };
 
+// 16 bytes from LDS to a row's values from `at` on, as far as it goes. The
+// whole piece is one vector, not four values: the compiler would share the
+// first value's store between both ways and split the piece.
+template <class T>
+__device__ __forceinline__ void store_piece(T* row, bool here, long at, long n,
+                                            const char* from) {
+  constexpr int N = 16 / sizeof(T);
+  typedef int Piece __attribute__((ext_vector_type(4), aligned(2)));
+  struct __attribute__((aligned(16))) Values { T v[N]; };
+  if (!here || at >= n) return;
+  if (at + N <= n) {
+    *(Piece*)(row + at) = *(const v4i*)from;
+  } else {
+    const Values w = *(const Values*)from;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (at + e < n) row[at + e] = w.v[e];
+  }
+}
+
 // Brings a tile's values into memory along its rows (or, ACROSS, along its
-// columns) by way of LDS, 16 of a wave's rows at a time, so that whole lines
-// are written: a wave by itself has 16 to 64 bytes of 16 rows (100,000 x 1000
-// float32 outputs: 101 us, written straight from the registers 155).
+// columns) by way of LDS, so that whole lines are written: from the registers
+// a wave has 16 to 64 bytes of 16 rows at a time. 100,000 x 1000 float32
+// outputs take 104 us so, written straight from the registers 155, and 140
+// with 16 rows in LDS at a time instead of as many as fit.
 //
 // value(i, j, v) gives the lane's four values of fragment (i, j), in PLANES
 // matrices; put(plane, row, column, at) stores 16 bytes that stand at `at`,
@@ -368,65 +389,98 @@ struct Tile {
 // `mine` for those that have values.
 template <class P, int BM, int BN, class V, int PLANES, bool ACROSS>
 struct Rows {
-  static constexpr int LONG = ACROSS ? BM : BN, SIDE = ACROSS ? BN : BM;
-  static constexpr int kCount = SIDE / (ACROSS ? P::kSpanN : P::kSpanM) * 16;
-  static constexpr int kPitch = LONG * (int)sizeof(V) + 16;  // shifts the banks
-  static constexpr int kPlane = kCount * kPitch;
-  // one is written while the other is stored, where there is room for two
-  static constexpr int kBuffers = 2 * PLANES * kPlane <= P::kLds ? 2 : 1;
-  static constexpr int kLds = kBuffers * PLANES * kPlane;
+  static constexpr int kSize = (int)sizeof(V);
+  static constexpr int kOuter = ACROSS ? P::NJ : P::MI;
+  static constexpr int kInner = ACROSS ? P::MI : P::NJ;
+  static constexpr int kSpan = ACROSS ? P::kSpanN : P::kSpanM;
+  // A wave whose own pieces of rows are whole lines needs no other wave.
+  static constexpr bool kAlone = !ACROSS && P::kSpanN * kSize >= 128;
+  // 16-byte pieces of a row, and 16 rows of every wave that shares them
+  static constexpr int kPieces =
+      (kAlone ? P::kSpanN : ACROSS ? BM : BN) * kSize / 16;
+  static constexpr int kWavesBeside = kAlone ? 1 : (ACROSS ? BN : BM) / kSpan;
+  static constexpr int kCount = kWavesBeside * 16;
+  // bank conflicts: pieces change places by row, or rows are a piece longer
+  static constexpr bool kTurned = (kPieces & (kPieces - 1)) == 0 && kAlone;
+  static constexpr int kPitch = (kPieces + !kTurned) * 16;
+  static constexpr int kOne = (kAlone ? P::kGroup : 1) * PLANES * kCount *
+                              kPitch;
+  static constexpr int kFit = P::kLds / kOne < kOuter ? P::kLds / kOne
+                                                      : kOuter;
+  static_assert(kFit > 0, "");
+  static constexpr int kRounds = (kOuter + kFit - 1) / kFit;
+  static constexpr int kRound = (kOuter + kRounds - 1) / kRounds;
+
+  static __device__ __forceinline__ int piece(int row, int k) {
+    return (kTurned ? k ^ (row & (kPieces - 1) & 7) : k) * 16;
+  }
+
   template <class Value, class Put>
   static __device__ __forceinline__ void store(char* lds, bool mine, int wm,
                                                int wn, Value value, Put put) {
-    static_assert(kLds <= P::kLds, "");
-    constexpr int OUTER = ACROSS ? P::NJ : P::MI;
-    constexpr int INNER = ACROSS ? P::MI : P::NJ;
-    constexpr int CHUNKS = LONG * (int)sizeof(V) / 16;
     const int lane = threadIdx.x & 63, c = lane & 15, h = lane >> 4;
-    // the wave's first of the rows that are together in LDS
-    const int base = ACROSS ? wn / P::kSpanN * 16 : wm / P::kSpanM * 16;
+    char* own = lds + (kAlone ? (threadIdx.x >> 6) * (PLANES * kRound *
+                                                      kCount * kPitch)
+                              : 0);
+    constexpr int kPlane = kRound * kCount * kPitch;
+    // the wave's first of 16 rows, and its first value in them
+    const int base = kAlone ? 0 : (ACROSS ? wn : wm) / kSpan * 16;
+    const int off = kAlone ? 0 : ACROSS ? wm : wn;
     auto turn = [] {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
+      // within a wave LDS goes in order
+      if (!kAlone) __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     };
-    turn();
+    __syncthreads();
+    if (kAlone && !mine) return;
 #pragma unroll
-    for (int o = 0; o < OUTER; ++o) {
-      char* buf = lds + o % kBuffers * PLANES * kPlane;
+    for (int o0 = 0; o0 < kOuter; o0 += kRound) {
       if (mine) {
 #pragma unroll
-        for (int u = 0; u < INNER; ++u) {
-          V v[PLANES][4];
-          if (ACROSS) value(u, o, v);
-          else value(o, u, v);
+        for (int o = o0; o < kOuter && o < o0 + kRound; ++o)
 #pragma unroll
-          for (int p = 0; p < PLANES; ++p) {
-            V* to = (V*)(buf + p * kPlane);
-            constexpr int PITCH = kPitch / (int)sizeof(V);
-            if (ACROSS) {
+          for (int u = 0; u < kInner; ++u) {
+            V v[PLANES][4];
+            if (ACROSS) value(u, o, v);
+            else value(o, u, v);
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                to[(base + h * 4 + r) * PITCH + wm + u * 16 + c] = v[p][r];
-            } else {
-              struct __attribute__((aligned(4 * sizeof(V)))) Four { V v[4]; };
-              *(Four*)(to + (base + c) * PITCH + wn + u * 16 + h * 4) =
-                  Four{v[p][0], v[p][1], v[p][2], v[p][3]};
+            for (int p = 0; p < PLANES; ++p) {
+              char* to = own + p * kPlane + (o - o0) * kCount * kPitch;
+              if (ACROSS) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  *(V*)(to + (base + h * 4 + r) * kPitch +
+                        (off + u * 16 + c) * kSize) = v[p][r];
+              } else {
+                struct __attribute__((aligned(4 * sizeof(V)))) Four {
+                  V v[4];
+                };
+                const int at = (off + u * 16 + h * 4) * kSize;
+                *(Four*)(to + (base + c) * kPitch + piece(c, at / 16) +
+                         at % 16) = Four{v[p][0], v[p][1], v[p][2], v[p][3]};
+              }
             }
           }
-        }
       }
       turn();
-      for (int k = threadIdx.x; k < kCount * CHUNKS; k += P::kThreads) {
-        const int r = k / CHUNKS, at = k % CHUNKS * 16;
-        const int row = r / 16 * (ACROSS ? P::kSpanN : P::kSpanM) + o * 16 +
-                        r % 16;
+      constexpr int kThreads = kAlone ? 64 : P::kThreads;
+      const int rows = min(kRound, kOuter - o0) * kCount;
+#pragma unroll 4
+      for (int k = kAlone ? lane : threadIdx.x; k < rows * kPieces;
+           k += kThreads) {
+        const int r = k / kPieces, at = k % kPieces;
+        const int in = r % kCount;  // of the 16 rows of each wave
+        const int row = (kAlone ? wm : in / 16 * kSpan) +
+                        (o0 + r / kCount) * 16 + in % 16;
 #pragma unroll
         for (int p = 0; p < PLANES; ++p)
-          put(p, row, at / (int)sizeof(V), buf + p * kPlane + r * kPitch + at);
+          put(p, row, (kAlone ? wn : 0) + at * (16 / kSize),
+              own + p * kPlane + r * kPitch + piece(in, at));
       }
-      if (kBuffers == 1) turn();
+      if (o0 + kRound < kOuter) turn();
     }
+    if (!kAlone) turn();
   }
 };
 
@@ -484,7 +538,7 @@ inline double tile_time(const TileCost& c, long tiles, long steps) {
 #define BY_TILE_SIZE_2(size, tiles, LAUNCH)               \
   switch (size) {                                         \
     case 256: LAUNCH(256, 128, 64, 2, 1, 1); break;       \
-    case 192: LAUNCH(192, 96, 48, 3, 1, 1); break;        \
+    case 192: LAUNCH(192, 96, 48, 2, 1, 2); break;        \
     case 128: LAUNCH(128, 64, 32, 3, 1, 2); break;        \
     case 96:                                              \
       if ((tiles) <= 256) LAUNCH(96, 48, 48, 4, 1, 2);    \
