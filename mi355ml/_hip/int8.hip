@@ -577,18 +577,23 @@ Plan plan_of(long m, long n, long k) {
     want = std::min(want, std::min(64L, std::max(1L, (long)steps / 16)));
     p.splits = (int)want;
   } else {
-    // the tile and the split that need the least time; joining the parts
-    // takes a launch, and writes and reads them at 4 TB/s
+    // The tile and the split that need the least time. Joining the parts
+    // takes a launch, and writes and reads them. Where the operands come from
+    // memory, 4 of 128 x 128's steps in LDS keep it busier than smaller tiles
+    // do (4096 x 50000 by 50, parts and all: 45 us, 64 x 64 51 us; 30000 rows
+    // of 30000 by 40: 158 us, 64 x 64 199 us). Over 21 products of 500 to
+    // 100,000 a side this choice costs 2.6% more than the best of all.
     double best = 1e30;
     for (const TileCost& c : kTiles[0])
       for (int splits = 1; splits <= 64 && splits <= (steps + 3) / 4;
            splits *= 2) {
         const long tm = (m + c.size - 1) / c.size;
         const long tn = (n + c.size - 1) / c.size;
+        const long tiles = tm * tn * splits;
         const int per = (steps + splits - 1) / splits;
-        const double join =
-            splits > 1 ? 4.0 + 8e-6 * splits * m * n / 4.0 : 0.0;
-        const double t = tile_time(c, tm * tn * splits, per) + join;
+        const double join = splits > 1 ? 3.0 + 1.5e-6 * splits * m * n : 0.0;
+        const double rate = c.size == 128 && tiles <= 256 ? 5.6e6 : 4.4e6;
+        const double t = tile_time(c, tiles, per, (m + n) * k / rate) + join;
         if (t < best) {
           best = t;
           p.size = c.size;

@@ -863,7 +863,8 @@ void step_as(Sources s, Step p, int batch, hipStream_t st) {
   int size = 0;
   double best = 0;
   for (const TileCost& c : kTiles[PARTS - 1]) {
-    const double t = tile_time(c, tiles_of(c.size) * batch, s.kbytes / kStep);
+    const double t = tile_time(c, tiles_of(c.size) * batch,
+                               s.kbytes / kStep, 0.0);
     if (!size || t < best) {
       size = c.size;
       best = t;

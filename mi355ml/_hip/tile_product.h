@@ -258,10 +258,6 @@ struct Tile {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[i][j] = ACC{0, 0, 0, 0};
 
-    // A step's two halves of 64 bytes are multiplied while the next half is
-    // on its way from LDS, across the turn of the buffers too: the matrix
-    // cores wait for nothing but the barrier. A buffer is loaded again right
-    // after the turn that frees it, a whole step before it is read.
     // A step's two halves are multiplied while the next half is on its way
     // from LDS, across the turn of the buffers too, so that the matrix cores
     // wait for nothing but the barrier (one a step). A buffer is loaded again
@@ -505,12 +501,14 @@ constexpr TileCost kTiles[3][kSizes] = {
     {{256, 5.4, 5.4, 20.0}, {192, 3.0, 3.3, 11.0}, {128, 1.5, 1.5, 4.5},
      {96, 0.92, 0.87, 2.8}, {64, 0.47, 0.43, 1.3}, {32, 0.32, 0.17, 0.5}}};
 
-// us for `tiles` tiles of `steps` steps
-inline double tile_time(const TileCost& c, long tiles, long steps) {
+// us for `tiles` tiles of `steps` steps, whose operands take `memory` us
+inline double tile_time(const TileCost& c, long tiles, long steps,
+                        double memory) {
   const double rounds = (double)((tiles + 255) / 256);
   const double step =
       rounds <= 1 || c.more * rounds < c.first ? c.first : c.more * rounds;
-  return step * steps + c.ends * rounds;
+  const double time = step * steps;
+  return (time > memory ? time : memory) + c.ends * rounds;
 }
 
 // LAUNCH(BM, WM, WN, STAGES, GROUPS, PARTS) for tiles of `size`. Up to 128,
@@ -538,7 +536,7 @@ inline double tile_time(const TileCost& c, long tiles, long steps) {
 #define BY_TILE_SIZE_2(size, tiles, LAUNCH)               \
   switch (size) {                                         \
     case 256: LAUNCH(256, 128, 64, 2, 1, 1); break;       \
-    case 192: LAUNCH(192, 96, 48, 2, 1, 2); break;        \
+    case 192: LAUNCH(192, 96, 48, 3, 1, 1); break;        \
     case 128: LAUNCH(128, 64, 32, 3, 1, 2); break;        \
     case 96:                                              \
       if ((tiles) <= 256) LAUNCH(96, 48, 48, 4, 1, 2);    \
