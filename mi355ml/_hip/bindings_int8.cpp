@@ -32,6 +32,9 @@ int type_id(torch::ScalarType t) {
   }
 }
 
+// 512 threads for 16 columns: with more a launch would pass 2^32 threads
+constexpr long kMostRows = 1L << 27;
+
 hipStream_t stream_of(const torch::Tensor& t) {
   return at::hip::getCurrentHIPStream(t.device().index()).stream();
 }
@@ -103,8 +106,7 @@ torch::Tensor int8_product(torch::Tensor xq, torch::Tensor xs,
   // 131071 products of at most 128^2 fit in 32 bits
   TORCH_CHECK(k < 131072, "k must be below 131072, so that the sums fit in "
               "32 bits (got ", k, ")");
-  TORCH_CHECK(m < (1L << 31) - 256 && n < (1L << 31) - 256,
-              "xq or wq has too many rows");
+  TORCH_CHECK(m < kMostRows && n < kMostRows, "xq or wq has too many rows");
   TORCH_CHECK(wq.device() == xq.device(), "wq must be on xq's device");
   const c10::DeviceGuard guard(xq.device());
   xs = vector_of(xs, m, xq.device(), "x_scale");
@@ -115,7 +117,7 @@ torch::Tensor int8_product(torch::Tensor xq, torch::Tensor xs,
   auto out = torch::empty({m, n}, xq.options().dtype(out_type));
   if (m == 0 || n == 0) return out;
   if (k == 0) {
-    if (b.defined()) out.copy_(b.expand({m, n})); else out.zero_();
+    if (b.defined()) out.copy_(b.detach().expand({m, n})); else out.zero_();
     return out;
   }
   xq = aligned_rows(xq);
@@ -148,7 +150,7 @@ torch::Tensor int8_linear(torch::Tensor x, torch::Tensor wq, torch::Tensor ws,
   }
   TORCH_CHECK(wq.dtype() == torch::kInt8 && wq.device() == x.device(),
               "wq must be int8 on x's device");
-  TORCH_CHECK(n < (1L << 31) - 256, "wq has too many rows");
+  TORCH_CHECK(n < kMostRows, "wq has too many rows");
   const int xtype = type_id(x.scalar_type()), type = type_id(out_type);
   const c10::DeviceGuard guard(x.device());
   ws = vector_of(ws, n, x.device(), "w_scale");

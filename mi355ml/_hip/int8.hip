@@ -250,9 +250,19 @@ void quantize_as(const T* x, long m, long k, long stride, int8_t* q,
                        st, x, m, (int)k, stride, q, qstride, scale);
 }
 
+// A launch holds fewer than 2^32 threads: rows that a workgroup takes one by
+// one go 2^23 at a time.
+constexpr long kRowsAtATime = 1 << 23;
+
 template <class T>
 void quantize(const T* x, long m, long k, long stride, int8_t* q,
               long qstride, float* scale, hipStream_t st) {
+  for (; m > kRowsAtATime; m -= kRowsAtATime) {
+    quantize(x, kRowsAtATime, k, stride, q, qstride, scale, st);
+    x += kRowsAtATime * stride;
+    q += kRowsAtATime * qstride;
+    scale += kRowsAtATime;
+  }
   // chunks of the padded row, so that its zeros are written too
   const long chunks = (qstride * (long)sizeof(T) + 15) / 16;
 #define ROWS(LANES, CH) \
@@ -510,7 +520,8 @@ __global__ __launch_bounds__(kLinearWaves * 64) void int8_linear_few_k(
     for (int i = 1; i < kLinearWaves; ++i) big = max_abs(big, part[r][i]);
     const RowScale rs(big);
     if (threadIdx.x == 0) scale[r] = rs.scale();
-    for (int at = threadIdx.x * VEC; at < steps * 128; at += kLinearWaves * 64 * VEC) {
+    for (int at = threadIdx.x * VEC; at < steps * 128;
+         at += kLinearWaves * 64 * VEC) {
       float v[VEC];
       uint32_t q[VEC / 4];
       load_chunk<TX, VEC>(x + r * stride, at, k, v);
@@ -590,6 +601,7 @@ Plan plan_of(long m, long n, long k) {
         const long tm = (m + c.size - 1) / c.size;
         const long tn = (n + c.size - 1) / c.size;
         const long tiles = tm * tn * splits;
+        if (tiles >= 1 << 23) continue;  // of at most 512 threads: 2^32
         const int per = (steps + splits - 1) / splits;
         const double join = splits > 1 ? 3.0 + 1.5e-6 * splits * m * n : 0.0;
         const double rate = c.size == 128 && tiles <= 256 ? 5.6e6 : 4.4e6;

@@ -104,7 +104,6 @@ struct Columns {
 // A wave takes 16 positions of the longer side at a time and has all tiles in
 // registers, the next 16 positions on their way.
 // ---------------------------------------------------------------------------
-// ---------------------------------------------------------------------------
 template <class T, int NT, bool WIDE>
 __device__ __forceinline__ void load_group(const Panel<T, WIDE>& panel,
                                            const Columns<NT>& columns, long g,

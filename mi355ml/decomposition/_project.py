@@ -22,9 +22,10 @@ def project(t: torch.Tensor, components: torch.Tensor, dtype: str,
     """t @ components.T, its columns times ``scale``.
 
     dtype "int8" holds the rows and the components in 8 bits, each with a
-    scale of its own, for the product: within about 0.5% of the norm of what
-    float32 gives, for a quarter of the bytes. ``scale`` goes into the
-    components' scales there.
+    scale of its own, for the product, at a quarter of the bytes. What float32
+    gives is met within about 1% of its norm where the rows are noise (0.8%
+    at 50 columns, 1.4% at 50,000), within 0.5% where they lie near the
+    components. ``scale`` goes into the components' scales there.
     """
     if dtype == "int8":
         vq, vs = quantize_rows(components.float())

@@ -10,7 +10,7 @@ its rows and one for each of its columns:
     y[i, j] = (sum_k xq[i, k] wq[j, k]) * x_scale[i] * w_scale[j] + bias[j]
 
 The sum is exact: it is taken in 32-bit integers, which k < 131072 values
-cannot overflow.
+cannot overflow. None of this is differentiable: results carry no gradient.
 """
 
 from __future__ import annotations
@@ -24,6 +24,8 @@ from ._ext import hip_ext, use_hip
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 #: the longest sum of products of 8-bit values that 32 bits always hold
 MAX_K = 131071
+#: most rows of either operand of a product
+MAX_ROWS = 2 ** 27 - 1
 
 
 def _check_floats(x: torch.Tensor, name: str) -> None:
@@ -50,6 +52,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     _check_floats(x, "x")
     if use_hip(x):
         return hip_ext().quantize_rows(x)
+    x = x.detach()
     if x.shape[1] == 0:
         return (torch.empty(x.shape, dtype=torch.int8, device=x.device),
                 torch.zeros(x.shape[0], device=x.device))
@@ -91,6 +94,10 @@ def _check_weights(x, x_name, wq, w_scale, bias, out_dtype) -> None:
     if x.shape[1] > MAX_K:
         raise ValueError(f"rows of more than {MAX_K} values could overflow "
                          f"the 32-bit sums, got {x.shape[1]}")
+    for name, rows in ((x_name, x.shape[0]), ("wq", wq.shape[0])):
+        if rows > MAX_ROWS:
+            raise ValueError(f"{name} may have at most {MAX_ROWS} rows, got "
+                             f"{rows}")
     if wq.device != x.device:
         raise ValueError(f"wq is on {wq.device}, the rows are on {x.device}")
     _check_vector(w_scale, wq.shape[0], x.device, "w_scale")
@@ -119,9 +126,9 @@ def int8_matmul(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor,
                                       out_dtype)
     # float64 holds every one of the integer sums
     y = (xq.double() @ wq.double().t()).float()
-    y = y * x_scale[:, None] * w_scale[None, :]
+    y = y * x_scale.detach()[:, None] * w_scale.detach()[None, :]
     if bias is not None:
-        y = y + bias
+        y = y + bias.detach()
     return y.to(out_dtype)
 
 

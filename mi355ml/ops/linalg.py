@@ -26,7 +26,7 @@ import torch
 from ..core.array import DistArray
 from ..core import random as mlrand
 from ._ext import hip_ext, use_hip
-from .orthogonalize import (COEFFICIENTS, MAX_PANEL, check_iteration,
+from .orthogonalize import (COEFFICIENTS, FLOATS, MAX_PANEL, check_iteration,
                             factor_of_gram)
 
 
@@ -166,6 +166,9 @@ def newton_schulz_panel(X: DistArray, steps: int = 5,
     c = check_iteration(steps, coefficients)
     a = X._as2d()
     d = a.shape[1]
+    if a.dtype not in FLOATS:
+        raise TypeError(f"a panel must be float32, float16 or bfloat16, got "
+                        f"{a.dtype}")
     if not 1 <= d <= MAX_PANEL:
         raise ValueError(f"a panel has 1 to {MAX_PANEL} columns, got {d}")
     comm = X.comm

@@ -22,7 +22,7 @@ import torch
 
 from ._ext import hip_ext, use_hip
 
-_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 #: most columns of a panel that is spread over ranks
 MAX_PANEL = 128
@@ -72,7 +72,7 @@ def newton_schulz(x: torch.Tensor, steps: int = 5,
     a, b, c = check_iteration(steps, coefficients)
     if x.dim() not in (2, 3):
         raise ValueError(f"x must be 2-D or 3-D, got {x.dim()}-D")
-    if x.dtype not in _FLOATS:
+    if x.dtype not in FLOATS:
         raise TypeError(f"x must be float32, float16 or bfloat16, got "
                         f"{x.dtype}")
     if use_hip(x):

@@ -492,3 +492,74 @@ def test_gpu_other_stream_and_graph():
         torch.cuda.synchronize()
         for _, out, m in graphs:
             assert torch.equal(out, ops.int8_linear(new[:m], wq, ws))
+
+
+def test_refuses_more_rows_than_a_launch_holds():
+    # nothing of this size is held: the rows are one, repeated
+    few = torch.zeros(1, 16, dtype=torch.int8)
+    many = few.expand(2 ** 27, 16)
+    one, ones = torch.ones(1), torch.ones(1).expand(2 ** 27)
+    with pytest.raises(ValueError, match="xq may have at most"):
+        ops.int8_matmul(many, ones, few, one)
+    with pytest.raises(ValueError, match="wq may have at most"):
+        ops.int8_matmul(few, one, many, ones)
+    with pytest.raises(ValueError, match="wq may have at most"):
+        ops.int8_linear(torch.zeros(1, 16), many, ones)
+
+
+def _check_no_gradient(device):
+    for k in (20, 0):
+        x = torch.randn(3, k, device=device, requires_grad=True)
+        q, s = ops.quantize_rows(x)
+        assert not s.requires_grad
+        b = torch.randn(3, device=device, requires_grad=True)
+        s.requires_grad_()
+        for y in (ops.int8_linear(x, q, s, b), ops.int8_matmul(q, s, q, s, b),
+                  ops.int8_linear(x, q.clone(), s)):
+            assert not y.requires_grad
+
+
+def test_results_carry_no_gradient():
+    _check_no_gradient("cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_results_carry_no_gradient():
+    _check_no_gradient("cuda")
+
+
+@pytest.mark.gpu
+def test_gpu_more_rows_than_one_launch_quantises():
+    # 1025 halves are taken a row by a workgroup of 256 threads: 2^24 rows
+    # would be 2^32 threads. The rows are one, repeated.
+    m, k = 2 ** 24 + 5, 1025
+    row = torch.randn(1, k, device="cuda", dtype=torch.float16)
+    q, s = ops.quantize_rows(row.expand(m, k))
+    want_q, want_s = ops.quantize_rows(row)
+    assert bool((s == want_s).all())
+    for lo, hi in ((0, 3), (2 ** 23 - 2, 2 ** 23 + 2), (m - 8, m)):
+        assert bool((q[lo:hi] == want_q).all())
+
+
+@pytest.mark.gpu
+def test_gpu_output_of_more_than_2_to_the_31_values():
+    m, n, k = 2 ** 26 + 77, 33, 20
+    g = torch.Generator(device="cuda").manual_seed(3)
+    xq = torch.randint(-127, 128, (m, 32), generator=g, device="cuda",
+                       dtype=torch.int8)[:, :k]
+    wq = torch.randint(-127, 128, (n, 32), generator=g, device="cuda",
+                       dtype=torch.int8)[:, :k]
+    xs, ws = torch.rand(m, device="cuda"), torch.rand(n, device="cuda")
+    y = ops.int8_matmul(xq, xs, wq, ws, out_dtype=torch.float16)
+    for lo in (0, 2 ** 31 // n - 100, m - 200):
+        rows = slice(lo, lo + 200)
+        want = ((xq[rows].cpu().double() @ wq.cpu().double().t()) *
+                xs[rows].cpu().double()[:, None] * ws.cpu().double())
+        # Roundings to 24 bits (the product with a scale, twice) and one to
+        # 11; subnormal results are off by half of 2^-24. Sums reach 20 * 127^2
+        # = 322580: what passes fp16's largest value becomes an infinity.
+        got = y[rows].cpu().double()
+        near = (got - want).abs() <= want.abs() * (2.0 ** -11 + 2.0 ** -21)
+        near |= (want.abs() < 2.0 ** -14) & ((got - want).abs() <= 2.0 ** -25)
+        near |= torch.isinf(got) & (want.abs() >= 65519.9)
+        assert bool(near.all())

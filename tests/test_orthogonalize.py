@@ -9,7 +9,7 @@ from mi355ml import ops
 from mi355ml.core.array import DistArray, from_numpy
 from mi355ml.decomposition import PCA, TruncatedSVD
 from mi355ml.ops.linalg import newton_schulz_panel, svd_compressed
-from mi355ml.ops.orthogonalize import COEFFICIENTS
+from mi355ml.ops.orthogonalize import COEFFICIENTS, factor_of_gram
 
 FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -365,3 +365,46 @@ def test_gpu_other_stream_and_graph():
         torch.cuda.synchronize()
         for (_, out), x in zip(graphs, new):
             assert torch.equal(out, ops.newton_schulz(x))
+
+
+def test_panel_refuses_other_types():
+    x = from_numpy(np.zeros((40, 5)))
+    assert x.dtype == torch.float64
+    with pytest.raises(TypeError, match="float32, float16 or bfloat16"):
+        newton_schulz_panel(x)
+
+
+def _by_gram(x, rows):
+    """Rows of X Q, X [m, k] and Q from the Gram matrix in 64 bits."""
+    gram = torch.zeros(x.shape[1], x.shape[1], dtype=torch.float64,
+                       device=x.device)
+    for part in x.split(1 << 20):
+        gram += part.double().t().contiguous() @ part.double()
+    q = factor_of_gram(gram, 5, COEFFICIENTS)
+    return torch.cat([x[r].double() for r in rows]) @ q
+
+
+@pytest.mark.gpu
+def test_gpu_panel_of_more_than_2_to_the_31_values():
+    m, k = 2 ** 31 // 60 + 3000, 60
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(m, k, generator=g, device="cuda")
+    rows = [slice(0, 500), slice(m // 2, m // 2 + 500), slice(m - 500, m)]
+    want = _by_gram(x, rows)
+    y = ops.newton_schulz(x)
+    got = torch.cat([y[r] for r in rows])
+    assert _far(got, want) <= _allowed(x, torch.float32, True)
+
+
+@pytest.mark.gpu
+def test_gpu_stack_of_more_than_2_to_the_31_values():
+    b, n, m = 17, 130, 1000004
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(b, n, m, generator=g, device="cuda",
+                    dtype=torch.bfloat16)
+    y = ops.newton_schulz(x)
+    rows = [slice(0, 300), slice(m - 300, m)]
+    for i in (0, b - 1):
+        want = _by_gram(x[i].t(), rows)
+        got = torch.cat([y[i].t()[r] for r in rows])
+        assert _far(got, want) <= _allowed(x, torch.bfloat16, False)
