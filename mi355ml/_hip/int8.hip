@@ -466,18 +466,27 @@ __global__ __launch_bounds__(256) void int8_few_rows_k(
   }
 }
 
+// A barrier for what is in LDS: loads from memory stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // The same for rows of x that are still floats, and few values altogether:
 // every workgroup quantises them for itself into LDS, which takes less time
-// than a launch of its own, while its first weights are on their way.
+// than a launch of its own, while its first weights are on their way. x is
+// loaded before them: loads come back in order.
 constexpr int kFewValues = 16384;  // m * k, k rounded up
 constexpr int kLinearWaves = 8;
 
 template <class TX, class T>
 __global__ __launch_bounds__(kLinearWaves * 64) void int8_linear_few_k(
     const TX* __restrict__ x, long stride, Sources s, Scales e) {
-  constexpr int VEC = 16 / sizeof(TX);
+  constexpr int VEC = 16 / sizeof(TX), THREADS = kLinearWaves * 64;
+  constexpr int MINE = kFewValues / VEC / THREADS;  // pieces for a thread
   __shared__ __attribute__((aligned(16))) char rows[kFewValues + 16 * 16];
-  __shared__ float part[16][kLinearWaves];
+  __shared__ unsigned most[16];
   __shared__ float scale[16];
   __shared__ v4i sums[kLinearWaves][64];
   const int lane = threadIdx.x & 63;
@@ -486,6 +495,18 @@ __global__ __launch_bounds__(kLinearWaves * 64) void int8_linear_few_k(
   const int steps = (k + 127) / 128, tail = k - (steps - 1) * 128;
   const int ld = steps * 128 + 16;  // rows side by side in the banks
   const int n0 = blockIdx.x * 16, chunk = lane >> 4;
+  // piece i of a thread, VEC values from `at` of row `of`; 16 lanes share a
+  // row
+  const int per = steps * 128 / VEC, pieces = m * per;
+  int of[MINE], at[MINE];
+  typename Chunk<TX, VEC>::Raw raw[MINE];
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    const int u = min(i * THREADS + (int)threadIdx.x, pieces - 1);
+    of[i] = u / per;
+    at[i] = (u - of[i] * per) * VEC;
+    raw[i] = load_raw<TX, VEC>(x + of[i] * stride, at[i], k);
+  }
   const char* pw = s.b[0] +
                    (long)min(n0 + (lane & 15), s.rows_b - 1) * s.row_b;
   // x is zero behind the row's end; there the weights are read from its
@@ -495,54 +516,56 @@ __global__ __launch_bounds__(kLinearWaves * 64) void int8_linear_few_k(
     return *(const v4i*)(pw + (t == steps - 1 && c >= tail
                                    ? 0 : (long)t * 128 + c));
   };
-  constexpr int AHEAD = 4;
+  // 8192 x 8192 weights and one row: 15.9 us, with 4 steps ahead 16.2, with 8
+  // 23.8; with x behind the weights 18.1
+  constexpr int AHEAD = 2;
   v4i w[AHEAD][2];
 #pragma unroll
   for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
       w[u][kk] = weights(min(wave + kLinearWaves * u, steps - 1), kk);
-  for (int r = 0; r < m; ++r) {
-    float big = 0.0f, v[VEC];
-    for (int at = threadIdx.x * VEC; at < k; at += kLinearWaves * 64 * VEC) {
-      load_chunk<TX, VEC>(x + r * stride, at, k, v);
+  if (threadIdx.x < 16) most[threadIdx.x] = 0;
+  lds_barrier();
+  // magnitudes compare as integers, NaN above infinity
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) big = max_abs(big, v[i]);
-    }
+  for (int i = 0; i < MINE; ++i) {
+    float v[VEC];
+    unsigned big = 0;
+    place_raw<TX, VEC>(raw[i], at[i], k, v);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) big = max_abs(big, __shfl_xor(big, d));
-    if (lane == 0) part[r][wave] = big;
+    for (int r = 0; r < VEC; ++r)
+      big = max(big, __float_as_uint(fabsf(v[r])));
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) big = max(big, __shfl_xor(big, d));
+    if ((lane & 15) == 0) atomicMax(&most[of[i]], big);
   }
-  __syncthreads();
-  for (int r = 0; r < m; ++r) {
-    float big = part[r][0];
+  lds_barrier();
 #pragma unroll
-    for (int i = 1; i < kLinearWaves; ++i) big = max_abs(big, part[r][i]);
-    const RowScale rs(big);
-    if (threadIdx.x == 0) scale[r] = rs.scale();
-    for (int at = threadIdx.x * VEC; at < steps * 128;
-         at += kLinearWaves * 64 * VEC) {
-      float v[VEC];
-      uint32_t q[VEC / 4];
-      load_chunk<TX, VEC>(x + r * stride, at, k, v);
-      rs.pack(v, q);
+  for (int i = 0; i < MINE; ++i) {
+    if (i * THREADS + (int)threadIdx.x >= pieces) continue;
+    float v[VEC];
+    uint32_t q[VEC / 4];
+    place_raw<TX, VEC>(raw[i], at[i], k, v);
+    RowScale(__uint_as_float(most[of[i]])).pack(v, q);
 #pragma unroll
-      for (int d = 0; d < VEC / 4; ++d)
-        ((uint32_t*)(rows + r * ld + at))[d] = q[d];
-    }
+    for (int d = 0; d < VEC / 4; ++d)
+      ((uint32_t*)(rows + of[i] * ld + at[i]))[d] = q[d];
   }
-  __syncthreads();
+  if (threadIdx.x < m)
+    scale[threadIdx.x] = RowScale(__uint_as_float(most[threadIdx.x])).scale();
+  lds_barrier();
   const char* px = rows + min(lane & 15, m - 1) * ld + chunk * 16;
   v4i acc = {0, 0, 0, 0};
   for (int t = wave; t < steps; t += kLinearWaves * AHEAD)
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int at = t + kLinearWaves * u;
-      if (at >= steps) break;
+      const int step = t + kLinearWaves * u;
+      if (step >= steps) break;
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        acc = mma(w[u][kk], *(const v4i*)(px + at * 128 + kk * 64), acc);
-        w[u][kk] = weights(min(at + kLinearWaves * AHEAD, steps - 1), kk);
+        acc = mma(w[u][kk], *(const v4i*)(px + step * 128 + kk * 64), acc);
+        w[u][kk] = weights(min(step + kLinearWaves * AHEAD, steps - 1), kk);
       }
     }
   sums[wave][lane] = acc;
@@ -690,10 +713,10 @@ extern "C" void launch_int8_product(const int8_t* xq, long xstride,
     product<__bf16>(s, e, p, slab, st);
 }
 
-// Whether x goes through int8_linear_few_k: few values, and weights that keep
-// the chip busy without splitting K.
+// Whether x goes through int8_linear_few_k: few values, rows of a piece at
+// least, and weights that keep the chip busy without splitting K.
 extern "C" int int8_linear_in_one(long m, long n, long k) {
-  return m <= 16 && m * ((k + 127) / 128 * 128) <= kFewValues &&
+  return m <= 16 && k >= 8 && m * ((k + 127) / 128 * 128) <= kFewValues &&
          plan_of(m, n, k).splits == 1;
 }
 
