@@ -38,30 +38,30 @@ template <> __device__ __forceinline__ float widen(__bf16 v) {
 constexpr float kLowBits = 12582912.0f;
 
 struct RowScale {
-  float s, inv;
+  float s, inv, up;
   bool fine, tiny;
   __device__ __forceinline__ RowScale(float big) {
     s = __fdiv_rn(big, 127.0f);
     fine = big < INFINITY;  // no infinity and no NaN
-    tiny = s < 1e-36f;      // 1 / s or x - q s would leave the normal range
-    inv = __fdiv_rn(1.0f, s);
+    // 1 / s or x - q s would leave the normal range: both times 2^64 first
+    tiny = s < 1e-36f;
+    up = tiny ? 0x1p64f : 1.0f;
+    inv = __fdiv_rn(1.0f, s * up);
   }
   __device__ __forceinline__ float scale() const { return fine ? s : NAN; }
   // every case, for one value
   __device__ __forceinline__ int slowly(float x) const {
-    if (!fine || s == 0.0f) return 0;
-    if (tiny) {
-      const double q = rint((double)x / (double)s);
-      return (int)fmin(127.0, fmax(-127.0, q));
-    }
-    float q = fmaf(x, inv, kLowBits) - kLowBits;
-    const float r = fmaf(-q, s, x);
-    const float a = fabsf(r), h = 0.5f * s;
-    if (a > h || (a == h && ((int)q & 1))) q += copysignf(1.0f, r);
-    return (int)q;
+    const float xu = x * up, su = s * up;
+    float q = fmaf(xu, inv, kLowBits) - kLowBits;
+    const float r = fmaf(-q, su, xu);
+    const float a = fabsf(r), h = 0.5f * su;
+    q += a > h || (a == h && ((int)q & 1)) ? copysignf(1.0f, r) : 0.0f;
+    // a subnormal s is rounded too coarsely to keep x / s below 127.5
+    return fine && s > 0.0f ? (int)fminf(127.0f, fmaxf(-127.0f, q)) : 0;
   }
   // N values to N bytes, N a multiple of 4: a product, a remainder and a
-  // maximum for a value, as long as none of them lies in the middle
+  // maximum for a value, as long as none of them lies in the middle (in
+  // 16-bit rows half the maximum does)
   template <int N>
   __device__ __forceinline__ void pack(const float (&x)[N],
                                        uint32_t (&w)[N / 4]) const {
@@ -84,10 +84,10 @@ struct RowScale {
   }
 };
 
-// NaN has to survive the maximum: fmaxf would drop it.
-__device__ __forceinline__ float max_abs(float m, float x) {
-  const float a = fabsf(x);
-  return (a > m || a != a) ? a : m;
+// Magnitudes compare as integers, and NaN, which fmaxf would drop, stands
+// above infinity.
+__device__ __forceinline__ unsigned max_abs(unsigned m, float x) {
+  return max(m, __float_as_uint(x) & 0x7fffffffu);
 }
 
 template <class T, int VEC> struct Chunk {
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256) void quantize_rows_k(
     int8_t* __restrict__ q, long qstride, float* __restrict__ scale) {
   constexpr int VEC = 16 / sizeof(T);
   constexpr int ROWS = 256 / LANES;
-  __shared__ float part[4];
+  __shared__ unsigned part[4];
   const int lane = threadIdx.x % LANES;
   const long first = (long)blockIdx.x * (ROWS * EACH) + threadIdx.x / LANES;
   float v[EACH][CH][VEC];
@@ -170,23 +170,23 @@ __global__ __launch_bounds__(256) void quantize_rows_k(
 #pragma unroll
   for (int r = 0; r < EACH; ++r) {
     const long row = first + r * ROWS;
-    float big = 0.0f;
+    unsigned big = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) big = max_abs(big, v[r][c][e]);
 #pragma unroll
     for (int d = 1; d < (LANES < 64 ? LANES : 64); d <<= 1)
-      big = max_abs(big, __shfl_xor(big, d));
+      big = max(big, __shfl_xor(big, d));
     if (LANES > 64) {
       if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = big;
       __syncthreads();
       big = part[0];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) big = max_abs(big, part[w]);
+      for (int w = 1; w < 4; ++w) big = max(big, part[w]);
     }
     if (row >= m) continue;
-    const RowScale rs(big);
+    const RowScale rs(__uint_as_float(big));
     if (lane == 0) scale[row] = rs.scale();
     int8_t* qr = q + row * qstride;
 #pragma unroll
@@ -207,23 +207,24 @@ __global__ __launch_bounds__(256) void quantize_long_rows_k(
     const T* __restrict__ x, long m, long k, long stride,
     int8_t* __restrict__ q, long qstride, float* __restrict__ scale) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ float part[4];
+  __shared__ unsigned part[4];
   const long row = blockIdx.x;
   const T* xr = x + row * stride;
-  float big = 0.0f, v[VEC];
+  float v[VEC];
+  unsigned big = 0;
   for (long at = (long)threadIdx.x * VEC; at < k; at += 256 * VEC) {
     load_chunk<T, VEC>(xr, at, k, v);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) big = max_abs(big, v[e]);
   }
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) big = max_abs(big, __shfl_xor(big, d));
+  for (int d = 1; d < 64; d <<= 1) big = max(big, __shfl_xor(big, d));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = big;
   __syncthreads();
   big = part[0];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) big = max_abs(big, part[w]);
-  const RowScale rs(big);
+  for (int w = 1; w < 4; ++w) big = max(big, part[w]);
+  const RowScale rs(__uint_as_float(big));
   if (threadIdx.x == 0) scale[row] = rs.scale();
   int8_t* qr = q + row * qstride;
   for (long at = (long)threadIdx.x * VEC; at < qstride; at += 256 * VEC) {
@@ -527,15 +528,13 @@ __global__ __launch_bounds__(kLinearWaves * 64) void int8_linear_few_k(
       w[u][kk] = weights(min(wave + kLinearWaves * u, steps - 1), kk);
   if (threadIdx.x < 16) most[threadIdx.x] = 0;
   lds_barrier();
-  // magnitudes compare as integers, NaN above infinity
 #pragma unroll
   for (int i = 0; i < MINE; ++i) {
     float v[VEC];
     unsigned big = 0;
     place_raw<TX, VEC>(raw[i], at[i], k, v);
 #pragma unroll
-    for (int r = 0; r < VEC; ++r)
-      big = max(big, __float_as_uint(fabsf(v[r])));
+    for (int r = 0; r < VEC; ++r) big = max_abs(big, v[r]);
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) big = max(big, __shfl_xor(big, d));
     if ((lane & 15) == 0) atomicMax(&most[of[i]], big);
