@@ -613,9 +613,9 @@ Plan plan_of(long m, long n, long k) {
     // The tile and the split that need the least time. Joining the parts
     // takes a launch, and writes and reads them. Where the operands come from
     // memory, 4 of 128 x 128's steps in LDS keep it busier than smaller tiles
-    // do (4096 x 50000 by 50, parts and all: 45 us, 64 x 64 51 us; 30000 rows
-    // of 30000 by 40: 158 us, 64 x 64 199 us). Over 21 products of 500 to
-    // 100,000 a side this choice costs 2.6% more than the best of all.
+    // do (4096 x 50000 by 50, parts and all: 45 us, 64 x 64 48 us; 30000 rows
+    // of 30000 by 40: 158 us, 64 x 64 167 us). Over 21 products of 500 to
+    // 100,000 a side this choice costs 3.5% more than the best of all.
     double best = 1e30;
     for (const TileCost& c : kTiles[0])
       for (int splits = 1; splits <= 64 && splits <= (steps + 3) / 4;

@@ -512,9 +512,11 @@ inline double tile_time(const TileCost& c, long tiles, long steps,
 }
 
 // LAUNCH(BM, WM, WN, STAGES, GROUPS, PARTS) for tiles of `size`. Up to 128,
-// where a CU gets one tile at most, as many steps in LDS as fit are quicker
-// (2048^2 outputs by 128: 39 us for 64 steps, with two 47), otherwise two, so
-// that several workgroups fit (4096^2 by 128: 144 us, with four 159).
+// as many steps in LDS as fit are quicker where a CU gets one tile at most
+// (2048^2 outputs by 128: 39 us for 64 steps, with two 47) or, by 64 and 96,
+// two (1500 x 700 by 64: 12.2 us for 24 steps, with two 14.7), otherwise two
+// steps, so that several workgroups fit (4096^2 by 128: 144 us, with four
+// 159).
 #define BY_TILE_SIZE_1(size, tiles, LAUNCH)               \
   switch (size) {                                         \
     case 256: LAUNCH(256, 128, 64, 2, 1, 1); break;       \
@@ -525,10 +527,11 @@ inline double tile_time(const TileCost& c, long tiles, long steps,
       break;                                              \
     case 96:                                              \
       if ((tiles) <= 256) LAUNCH(96, 48, 48, 4, 2, 1);    \
+      else if ((tiles) <= 512) LAUNCH(96, 48, 48, 3, 1, 1); \
       else LAUNCH(96, 48, 48, 2, 1, 1);                   \
       break;                                              \
     case 64:                                              \
-      if ((tiles) <= 256) LAUNCH(64, 32, 32, 4, 2, 1);    \
+      if ((tiles) <= 512) LAUNCH(64, 32, 32, 4, 2, 1);    \
       else LAUNCH(64, 32, 32, 2, 1, 1);                   \
       break;                                              \
     default: LAUNCH(32, 16, 16, 4, 1, 1);                 \
