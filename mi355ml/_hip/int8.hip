@@ -135,7 +135,8 @@ __device__ __forceinline__ void load_chunk(const T* row, long at, long k,
 // A row for LANES lanes, each holding CH chunks of 16 bytes of it between the
 // two passes (maximum, then rounding), so that x is read once; EACH rows at a
 // time for a lane, so that enough loads are on their way. Memory-bound: about
-// ten operations a value against the 5 (or 3) bytes that it moves.
+// ten operations a value against the 5 (or 3) bytes that it moves (10^6 x 100
+// float32: 88 us, 5.7 TB/s).
 template <class T, int LANES, int CH, int EACH>
 __global__ __launch_bounds__(256) void quantize_rows_k(
     const T* __restrict__ x, long m, int k, long stride,
@@ -517,8 +518,8 @@ __global__ __launch_bounds__(kLinearWaves * 64) void int8_linear_few_k(
     return *(const v4i*)(pw + (t == steps - 1 && c >= tail
                                    ? 0 : (long)t * 128 + c));
   };
-  // 8192 x 8192 weights and one row: 15.9 us, with 4 steps ahead 16.2, with 8
-  // 23.8; with x behind the weights 18.1
+  // 8192 x 8192 weights and one row: 15.4 us, 4.3 TB/s; with 4 steps ahead
+  // 0.3 us more, with 8 8 us; with x behind the weights 18.1
   constexpr int AHEAD = 2;
   v4i w[AHEAD][2];
 #pragma unroll

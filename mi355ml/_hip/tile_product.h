@@ -94,10 +94,10 @@ template <int N> struct Count { static constexpr int value = N; };
 // three parts by 64: 15 us, joined 25; 2048^2 by 128: 48, joined 58). Larger
 // tiles do not have the LDS, and gain nothing by it.
 //
-// At 4096^3 a product of fp16 runs at 1.2 PFLOP/s and one of int8 at 2.6 POP/s
-// (the library: 1.1 and 2.05). There the matrix cores are busy 60% of the time
-// at a clock that the power limit holds at 1.75 GHz; LDS is at a quarter of
-// its rate. Small tiles are bound by what a CU takes in: a step of 64 x 64
+// At 4096^3 a product of fp16 runs at 1.2 PFLOP/s (the library: 1.1) and one
+// of int8 at 2.1 POP/s (2.05), at 8192^3 at 2.54 (2.52). There the matrix
+// cores are busy 78% of the time at a clock that the power limit holds at
+// 1.75 GHz; LDS is at a quarter of its rate. Small tiles are bound by what a CU takes in: a step of 64 x 64
 // is 16 KB in 520 clocks, of about 40 B a clock that loads alone reach.
 template <class ACC, int BM, int BN, int WM, int WN, int STAGES, int GROUPS,
           int PARTS>
