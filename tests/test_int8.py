@@ -563,3 +563,31 @@ def test_gpu_output_of_more_than_2_to_the_31_values():
         near |= (want.abs() < 2.0 ** -14) & ((got - want).abs() <= 2.0 ** -25)
         near |= torch.isinf(got) & (want.abs() >= 65519.9)
         assert bool(near.all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [
+    # each size of tile with up to 256 of them, up to 512 and more, of one
+    # step, of a few and of many, with K whole and split
+    (130, 33, 5), (65, 1, 5001), (2049, 99, 5), (3001, 1, 20001),
+    (500, 2050, 100), (1000, 513, 129), (333, 101, 20001), (333, 4099, 5),
+    (1500, 1001, 700), (2049, 33, 20001), (500, 4099, 129),
+    (2049, 513, 20001), (2049, 1001, 300), (500, 301, 20001),
+    (1000, 4099, 129), (4100, 1001, 1300), (1500, 4099, 5),
+    (3001, 2050, 129), (777, 4099, 100), (1000, 303, 20001),
+    (9000, 2051, 100), (500, 4099, 20001), (2049, 4099, 129),
+    (2049, 2050, 20001), (4100, 4099, 300), (3001, 4099, 1300)])
+def test_gpu_product_choices(m, n, k, dtype):
+    g = torch.Generator(device="cuda").manual_seed(n)
+    xq, wq = (torch.randint(-127, 128, s, generator=g, device="cuda",
+                            dtype=torch.int8) for s in ((m, k), (n, k)))
+    xs, ws, b = (torch.rand(s, generator=g, device="cuda")
+                 for s in (m, n, n))
+    want, size = _product_expected(xq, xs, wq, ws, b)
+    got = ops.int8_matmul(xq, xs, wq, ws, b, dtype).double()
+    # four roundings in float32, and one to the result's type
+    half, last = 2.0 ** -24, torch.finfo(dtype).eps / 2
+    allowed = 4 * half * size * (1 + 8 * half)
+    assert ((got - want).abs() <= allowed + last * (want.abs() + allowed)
+            ).all()

@@ -408,3 +408,15 @@ def test_gpu_stack_of_more_than_2_to_the_31_values():
         want = _by_gram(x[i].t(), rows)
         got = torch.cat([y[i].t()[r] for r in rows])
         assert _far(got, want) <= _allowed(x, torch.bfloat16, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(17, 129, 700), (17, 4001, 129),
+                                   (17, 200, 2700), (17, 1500, 200),
+                                   (8, 140, 2700), (2, 129, 2700)])
+def test_gpu_stacks_of_many_tiles(shape, dtype):
+    # more tiles of a size than the chip holds at a time
+    x = _matrix(*shape, dtype=dtype).cuda()
+    far = _far(ops.newton_schulz(x), _iterate(x, torch.float64))
+    assert far <= _allowed(x, dtype, False), far
